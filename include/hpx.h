@@ -351,6 +351,76 @@ int hpx_dgc_decode(int count, const uint8_t* const* ins, const int32_t* in_sizes
                    float* const* outs, const int32_t* out_sizes,
                    const int32_t* is_add_tos, hpx_stream_t stream);
 
+/* ---- gradients before and after the codecs -----------------------------------
+ * No counterpart in the reference, whose caller does this in torch: the global
+ * norm of a list of gradients and clipping by it, and for the sparsifier above
+ * the two steps that keep the momentum of a sparsified gradient right (Lin et
+ * al. 2018, Deep Gradient Compression: momentum correction, momentum factor
+ * masking).
+ *   types      the element type of each gradient, NULL: all are HPX_F32.
+ *              Tensors start at any multiple of their element size.
+ *   result     HPX_GRAD_RESULT doubles of device memory that the caller owns and
+ *              has zeroed once: [0] S, [1] norm, [2] coefficient, the rest room
+ *              for the calls (zeroing it again is never needed).  A call in flight
+ *              has its block to itself; calls with blocks of their own, also
+ *              graphs captured on one stream, share nothing.
+ *   order      2: S = sum of squares over all tensors, N = sqrt(S);
+ *              HPX_NORM_MAX: S = N = the largest magnitude.  S is computed and
+ *              kept in fp64; its bits depend on the types, sizes and values of the
+ *              list alone, not on addresses or timing.  A NaN anywhere gives NaN.
+ *   coefficient c = scale * min(1, max_norm / (|scale| N + 1e-6)), rounded to
+ *              fp32 once; N that is infinite or a NaN gives c = 0.  max_norm may be
+ *              infinity (no clipping).  c = 0 takes nothing of a gradient, whatever it
+ *              holds: infinities and NaN times 0 are 0 here, so that a step that
+ *              overflowed does not reach residuals and momenta.
+ * The calls only enqueue kernels: no allocation, no wait, no workspace; all of
+ * them can be recorded into a graph. */
+#define HPX_F32 0
+#define HPX_BF16 1
+#define HPX_F16 2
+#define HPX_NORM_MAX 0
+#define HPX_GRAD_RESULT 2064
+
+/* result[0] = S, result[1] = N over the list.  is_add_to != 0: S of the list
+ * joins what result[0] holds (further lists; a NaN or negative value there is the
+ * caller's).  A norm over several ranks: all-reduce result[0] (sum, or
+ * maximum), then pass it on with is_measured. */
+int hpx_grad_norm(int count, const void* const* grads, const int64_t* sizes,
+                  const int32_t* types, int order, int is_add_to, double* result,
+                  hpx_stream_t stream);
+
+/* out = c * g for every element.  outs == NULL: in place, in the gradient's own
+ * type; with c = 1 nothing is touched.  Otherwise outs[t] is fp32 - what the
+ * codecs encode - and may be grads[t] where that is fp32.  is_measured == 0: the
+ * norm of this list is taken first, as by hpx_grad_norm; otherwise result[0] holds
+ * S already.  result[1] = |scale| N, result[2] = c.  -3 if two tensors that are
+ * written overlap, or one that is written and another gradient. */
+int hpx_grad_clip(int count, const void* const* grads, const int64_t* sizes,
+                  const int32_t* types, float* const* outs, int is_measured, int order,
+                  double max_norm, double scale, double* result, hpx_stream_t stream);
+
+/* Momentum correction: momenta[t] = momentum * momenta[t] + c * g, and with outs
+ * (not NULL) Nesterov's direction outs[t] = momentum * momenta[t] + c * g of the new
+ * momenta; c g is rounded once, the sum once more.  What goes to hpx_gd_encode as
+ * the gradient is momenta[t], or outs[t].  The coefficient is taken from result[0], as
+ * hpx_grad_norm and perhaps an all-reduce have left it, and told in result[1] and
+ * result[2]; result == NULL: c = scale.  momenta and outs are fp32; outs[t] may be
+ * grads[t] where that is fp32.  -3 if tensors overlap otherwise, as above. */
+int hpx_gd_momentum(int count, const void* const* grads, const int64_t* sizes,
+                    const int32_t* types, float* const* momenta, float* const* outs,
+                    float momentum, int order, double max_norm, double scale,
+                    double* result, hpx_stream_t stream);
+
+/* Momentum factor masking: momenta[t][i] = 0 for every index i that the message
+ * ins[t] (of hpx_gd_encode or hpx_dgc_encode) carries.  The header is read on the
+ * device; in_sizes[t] is the message's room.  Indices outside [0, sizes[t]) are
+ * passed over; a message whose header is not 4 + 8k or exceeds in_sizes[t] masks
+ * nothing.  counts: NULL, or `count` device words that get the number of entries
+ * of each message, -1 for such a header. */
+int hpx_gd_mask(int count, const uint8_t* const* ins, const int32_t* in_sizes,
+                float* const* momenta, const int32_t* sizes, int32_t* counts,
+                hpx_stream_t stream);
+
 /* ---- ECQ: error-compensated quantiser with a history -----------------------
  * The reference holds this codec as a body without a driver or a caller
  * (ecq_body / ecq_r_body, ecq_body.h:157-286 / :342-423); these two entry points

@@ -38,6 +38,10 @@ SYMBOLS = (
     "hpx_gd_fallbacks",
     "hpx_dgc_encode",
     "hpx_dgc_decode",
+    "hpx_grad_norm",
+    "hpx_grad_clip",
+    "hpx_gd_momentum",
+    "hpx_gd_mask",
     "hpx_ecq_encode",
     "hpx_ecq_decode",
     "hpx_powersgd_encode1",
@@ -68,6 +72,11 @@ class Task(C.Structure):
                 ("M", C.c_void_p), ("P", C.c_void_p), ("Q", C.c_void_p),
                 ("n", C.c_int32), ("m", C.c_int32), ("r", C.c_int32)]
 
+
+# constants of include/hpx.h
+F32, BF16, F16 = 0, 1, 2
+NORM_MAX = 0
+GRAD_RESULT = 2064
 
 _lib = None
 
@@ -115,6 +124,10 @@ def load():
     L.hpx_gd_decode.argtypes = [i32, pp, p, pp, p, p, p]
     L.hpx_dgc_encode.argtypes = [i32, pp, p, pp, p, p, p, p]
     L.hpx_dgc_decode.argtypes = [i32, pp, p, pp, p, p, p]
+    L.hpx_grad_norm.argtypes = [i32, pp, p, p, i32, i32, p, p]
+    L.hpx_grad_clip.argtypes = [i32, pp, p, p, pp, i32, i32, C.c_double, C.c_double, p, p]
+    L.hpx_gd_momentum.argtypes = [i32, pp, p, p, pp, pp, C.c_float, i32, C.c_double, C.c_double, p, p]
+    L.hpx_gd_mask.argtypes = [i32, pp, p, pp, p, p, p]
     L.hpx_ecq_encode.argtypes = [i32, pp, p, pp, pp, p, p, p, p, p, p]
     L.hpx_ecq_decode.argtypes = [i32, pp, p, pp, p, p, p]
     L.hpx_powersgd_encode1.argtypes = [i32, pp, p, pp, pp, pp, pp, p, p, p, p]

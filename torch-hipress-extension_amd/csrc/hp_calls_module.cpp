@@ -284,6 +284,183 @@ PyObject* powersgd_decode(PyObject* const* a) {  // Ps, Qs, Ms, residuals, grads
   return released([&] { return hpx_powersgd_decode(int(n), ro(pp), ro(qp), mp.data(), rp.data(), gp.data(), numel.data(), d.n.data(), d.m.data(), d.r.data(), st); });
 }
 
+// The gradients of a list, which may be of several types: addresses, sizes and type codes.  Tensors bring their type, and are
+// checked against `sizes` and the current device; an address is of the type that `types` gives (None: fp32), which a tensor
+// has to agree with.
+struct Grads {
+  std::vector<void*> p;
+  std::vector<int64_t> size;
+  std::vector<int32_t> type;
+};
+
+int32_t type_code(at::ScalarType t, const char* what) {
+  if (t == at::kFloat) return HPX_F32;
+  if (t == at::kBFloat16) return HPX_BF16;
+  if (t == at::kHalf) return HPX_F16;
+  PyErr_Format(PyExc_TypeError, "%s must be float32, bfloat16 or float16", what);
+  throw PyError{};
+}
+
+// A tensor among the elements of a list: of `size` elements at least, on the current device.
+void fits(const at::Tensor& t, int64_t size, const char* what) {
+  if (!t.is_cuda()) {
+    PyErr_Format(PyExc_RuntimeError, "%s must be a CUDA tensor", what);
+    throw PyError{};
+  }
+  if (t.get_device() != c10::hip::current_device()) {
+    PyErr_Format(PyExc_RuntimeError, "%s is on device %d, the current device is %d", what, int(t.get_device()), int(c10::hip::current_device()));
+    throw PyError{};
+  }
+  if (!t.is_contiguous()) {
+    PyErr_Format(PyExc_RuntimeError, "%s must be contiguous", what);
+    throw PyError{};
+  }
+  if (t.numel() < size) {
+    PyErr_Format(PyExc_ValueError, "%s has %lld elements, %lld are asked for", what, static_cast<long long>(t.numel()), static_cast<long long>(size));
+    throw PyError{};
+  }
+}
+
+Grads gradients(PyObject* list, PyObject* sizes, PyObject* types) {
+  Seq s(list);
+  Grads g;
+  g.size = ints<int64_t>(sizes, s.n, "sizes");
+  g.p.resize(size_t(s.n));
+  g.type.assign(size_t(s.n), HPX_F32);
+  if (types != Py_None) {
+    Seq t(types);
+    need(t.n, s.n, "types");
+    for (Py_ssize_t i = 0; i < s.n; i++)
+      g.type[size_t(i)] = THPDtype_Check(t.items[i]) ? type_code(reinterpret_cast<THPDtype*>(t.items[i])->scalar_type, "gradients") : static_cast<int32_t>(as_int(t.items[i]));
+  }
+  for (Py_ssize_t i = 0; i < s.n; i++) {
+    if (THPVariable_Check(s.items[i])) {
+      const at::Tensor& t = THPVariable_Unpack(s.items[i]);
+      const int32_t code = type_code(t.scalar_type(), "gradients");
+      fits(t, g.size[size_t(i)], "a gradient");
+      if (types != Py_None && code != g.type[size_t(i)]) {
+        PyErr_Format(PyExc_TypeError, "gradient %zd is not of the type that is given for it", i);
+        throw PyError{};
+      }
+      g.type[size_t(i)] = code;
+      g.p[size_t(i)] = t.data_ptr();
+    } else {
+      g.p[size_t(i)] = reinterpret_cast<void*>(static_cast<uintptr_t>(as_int(s.items[i])));
+    }
+  }
+  return g;
+}
+
+// The tensors of a list beside the gradients (or messages), all of one type: `size[i]` elements each.
+template <typename T, typename N>
+std::vector<T*> companions(PyObject* list, const std::vector<N>& size, size_t count, at::ScalarType type, const char* what) {
+  Seq s(list);
+  need(s.n, Py_ssize_t(count), what);
+  std::vector<T*> v(count);
+  for (size_t i = 0; i < count; i++) {
+    PyObject* o = s.items[i];
+    if (THPVariable_Check(o)) {
+      const at::Tensor& t = THPVariable_Unpack(o);
+      if (t.scalar_type() != type) {
+        PyErr_Format(PyExc_TypeError, "%s must be of type %s", what, c10::toString(type));
+        throw PyError{};
+      }
+      fits(t, int64_t(size[i]), what);
+      v[i] = static_cast<T*>(t.data_ptr());
+    } else {
+      v[i] = reinterpret_cast<T*>(static_cast<uintptr_t>(as_int(o)));
+    }
+  }
+  return v;
+}
+
+double* result_block(PyObject* o) {
+  if (!THPVariable_Check(o)) return reinterpret_cast<double*>(static_cast<uintptr_t>(as_int(o)));
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.scalar_type() != at::kDouble) {
+    PyErr_SetString(PyExc_TypeError, "the result block must be of type Double");
+    throw PyError{};
+  }
+  fits(t, HPX_GRAD_RESULT, "the result block");
+  return static_cast<double*>(t.data_ptr());
+}
+
+// The C call's refusals (-3) as a ValueError that carries its text, anything else as a RuntimeError.
+template <typename F>
+PyObject* released_or_raised(F&& call) {
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = call();
+  Py_END_ALLOW_THREADS
+  if (rc == HPX_OK) Py_RETURN_NONE;
+  PyErr_SetString(rc == HPX_ERR_ARG ? PyExc_ValueError : PyExc_RuntimeError, hpx_last_error());
+  throw PyError{};
+}
+
+int as_flag(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyError{};
+  return v;
+}
+
+PyObject* grad_norm(PyObject* const* a) {  // grads, sizes, result, order, is_add_to, types, stream
+  const Grads g = gradients(a[0], a[1], a[5]);
+  double* result = result_block(a[2]);
+  const int order = int(as_int(a[3])), add = as_flag(a[4]);
+  hipStream_t st = stream_of(a[6]);
+  return released_or_raised([&] { return hpx_grad_norm(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), order, add, result, st); });
+}
+
+PyObject* grad_clip(PyObject* const* a) {  // grads, sizes, outs, max_norm, result, is_measured, order, scale, types, stream
+  const Grads g = gradients(a[0], a[1], a[8]);
+  std::vector<float*> out;
+  if (a[2] != Py_None) out = companions<float>(a[2], g.size, g.p.size(), at::kFloat, "an output");
+  float* const* outs = a[2] != Py_None ? out.data() : nullptr;
+  const double max_norm = as_float(a[3]), scale = as_float(a[7]);
+  double* result = result_block(a[4]);
+  const int measured = as_flag(a[5]), order = int(as_int(a[6]));
+  hipStream_t st = stream_of(a[9]);
+  return released_or_raised([&] { return hpx_grad_clip(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), outs, measured, order, max_norm, scale, result, st); });
+}
+
+PyObject* gd_momentum(PyObject* const* a) {  // grads, sizes, momenta, outs, momentum, max_norm, result, order, scale, types, stream
+  const Grads g = gradients(a[0], a[1], a[9]);
+  const auto u = companions<float>(a[2], g.size, g.p.size(), at::kFloat, "a momentum");
+  std::vector<float*> out;
+  if (a[3] != Py_None) out = companions<float>(a[3], g.size, g.p.size(), at::kFloat, "an output");
+  float* const* outs = a[3] != Py_None ? out.data() : nullptr;
+  const double m = as_float(a[4]), max_norm = as_float(a[5]), scale = as_float(a[8]);
+  double* result = a[6] != Py_None ? result_block(a[6]) : nullptr;
+  const int order = int(as_int(a[7]));
+  hipStream_t st = stream_of(a[10]);
+  return released_or_raised(
+      [&] { return hpx_gd_momentum(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), u.data(), outs, float(m), order, max_norm, scale, result, st); });
+}
+
+PyObject* gd_mask(PyObject* const* a) {  // ins, in_sizes, momenta, sizes, counts, stream
+  Seq s(a[0]);
+  const size_t n = size_t(s.n);
+  const auto in_size = ints<int32_t>(a[1], s.n, "in sizes"), size = ints<int32_t>(a[3], s.n, "sizes");
+  const auto in = companions<uint8_t>(a[0], in_size, n, at::kByte, "a message");
+  const auto u = companions<float>(a[2], size, n, at::kFloat, "a momentum");
+  int32_t* counts = nullptr;
+  if (a[4] != Py_None) {
+    if (THPVariable_Check(a[4])) {
+      const at::Tensor& t = THPVariable_Unpack(a[4]);
+      if (t.scalar_type() != at::kInt) {
+        PyErr_SetString(PyExc_TypeError, "the counts must be of type Int");
+        throw PyError{};
+      }
+      fits(t, int64_t(n), "the counts");
+      counts = static_cast<int32_t*>(t.data_ptr());
+    } else {
+      counts = reinterpret_cast<int32_t*>(static_cast<uintptr_t>(as_int(a[4])));
+    }
+  }
+  hipStream_t st = stream_of(a[5]);
+  return released_or_raised([&] { return hpx_gd_mask(int(n), ro(in), in_size.data(), u.data(), size.data(), counts, st); });
+}
+
 // A fixed number of positional arguments, and C++ exceptions turned into Python ones.
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t ARGS>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -313,9 +490,13 @@ PyMethodDef g_methods[] = {
     method<powersgd_encode1, 6>("powersgd_encode1"),
     method<powersgd_encode2, 4>("powersgd_encode2"),
     method<powersgd_decode, 6>("powersgd_decode"),
+    method<grad_norm, 7>("grad_norm"),
+    method<grad_clip, 10>("grad_clip"),
+    method<gd_momentum, 11>("gd_momentum"),
+    method<gd_mask, 6>("gd_mask"),
     {nullptr, nullptr, 0, nullptr}};
 
-PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_hp_calls", "the nine hp_cuda_* drivers' argument lists, laid out natively", -1, g_methods,
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_hp_calls", "the argument lists of the hp_cuda_* drivers and gradient operators, laid out natively", -1, g_methods,
                         nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
