@@ -22,11 +22,15 @@ using namespace hpx;
 constexpr int kThreads = 256;
 
 // ---- the result block --------------------------------------------------------
-// doubles: [0] S, [1] norm, [2] coefficient, [3] arrivals (zero between calls), [16 ...] one partial sum per workgroup
+// doubles: [0] S, [1] norm, [2] coefficient, [3] arrivals, [16 ...] a partial sum per workgroup, then the arrivals of each group
+// of workgroups, a cache line each.  All arrivals are zero between calls.
 constexpr int kArrivals = 3;
 constexpr int kSlots = 16;
-constexpr int kMaxGrid = HPX_GRAD_RESULT - kSlots;
-static_assert(kMaxGrid == 2048, "eight workgroups of 256 lanes on each of 256 CUs");
+constexpr int kMaxGrid = 1024;  // four workgroups on each of 256 CUs
+constexpr int kGroups = 16;
+constexpr int kGroupArrivals = kSlots + kMaxGrid;
+constexpr int kLineDoubles = 16;
+static_assert(kGroupArrivals + kGroups * kLineDoubles <= HPX_GRAD_RESULT, "result block too small");
 
 // ---- tables ------------------------------------------------------------------
 // An element count and its type share a word: the count needs 48 bits.
@@ -49,7 +53,7 @@ struct ClipSeg {
 struct MomentumSeg {
   const void* g;
   float* u;
-  float* d;  // null: no direction
+  float* d;
   uint64_t nt;
   static constexpr int kCapLarge = 256;
 };
@@ -100,21 +104,49 @@ struct Elem<HPX_F16> {
 // Four consecutive elements as they lie in memory; a tensor may start at any element.
 template <typename Raw>
 struct __attribute__((packed, aligned(sizeof(Raw)))) Raw4 {
-  Raw v[4];
+  uint32_t w[sizeof(Raw)];
 };
 template <int TYPE>
-__device__ __forceinline__ float4 load4(const void* base, int64_t e) {
-  using E = Elem<TYPE>;
-  const Raw4<typename E::raw> r = *reinterpret_cast<const Raw4<typename E::raw>*>(static_cast<const typename E::raw*>(base) + e);
-  return make_float4(E::to(r.v[0]), E::to(r.v[1]), E::to(r.v[2]), E::to(r.v[3]));
+using raw4 = Raw4<typename Elem<TYPE>::raw>;
+
+template <int TYPE>
+__device__ __forceinline__ raw4<TYPE> load4(const void* base, int64_t e) {
+  return *reinterpret_cast<const raw4<TYPE>*>(static_cast<const typename Elem<TYPE>::raw*>(base) + e);
+}
+// Streaming forms (see ld4_stream): 138 M elements of momentum correction take 258 us with both, 297 with plain loads, 300 with
+// plain loads and stores.
+template <int TYPE>
+__device__ __forceinline__ raw4<TYPE> load4_stream(const void* base, int64_t e) {
+  const raw4<TYPE>* q = reinterpret_cast<const raw4<TYPE>*>(static_cast<const typename Elem<TYPE>::raw*>(base) + e);
+  raw4<TYPE> r;
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(typename Elem<TYPE>::raw); i++) r.w[i] = __builtin_nontemporal_load(&q->w[i]);
+  return r;
 }
 template <int TYPE>
-__device__ __forceinline__ void store4(void* base, int64_t e, float4 x) {
+__device__ __forceinline__ void store4_stream(void* base, int64_t e, float4 x) {
   using E = Elem<TYPE>;
-  Raw4<typename E::raw> r;
-  r.v[0] = E::from(x.x); r.v[1] = E::from(x.y); r.v[2] = E::from(x.z); r.v[3] = E::from(x.w);
-  *reinterpret_cast<Raw4<typename E::raw>*>(static_cast<typename E::raw*>(base) + e) = r;
+  uint32_t w[sizeof(typename E::raw)];
+  if constexpr (TYPE == HPX_F32) {
+    w[0] = E::from(x.x); w[1] = E::from(x.y); w[2] = E::from(x.z); w[3] = E::from(x.w);
+  } else {
+    w[0] = E::from(x.x) | uint32_t(E::from(x.y)) << 16;
+    w[1] = E::from(x.z) | uint32_t(E::from(x.w)) << 16;
+  }
+  raw4<TYPE>* q = reinterpret_cast<raw4<TYPE>*>(static_cast<typename E::raw*>(base) + e);
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(typename E::raw); i++) __builtin_nontemporal_store(w[i], &q->w[i]);
 }
+template <int TYPE>
+__device__ __forceinline__ float4 value4(const raw4<TYPE>& r) {
+  using E = Elem<TYPE>;
+  if constexpr (TYPE == HPX_F32) return make_float4(E::to(r.w[0]), E::to(r.w[1]), E::to(r.w[2]), E::to(r.w[3]));
+  else return make_float4(E::to(uint16_t(r.w[0])), E::to(uint16_t(r.w[0] >> 16)), E::to(uint16_t(r.w[1])), E::to(uint16_t(r.w[1] >> 16)));
+}
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* base, int64_t e) { return Elem<TYPE>::to(static_cast<const typename Elem<TYPE>::raw*>(base)[e]); }
+template <int TYPE>
+__device__ __forceinline__ void store1(void* base, int64_t e, float x) { static_cast<typename Elem<TYPE>::raw*>(base)[e] = Elem<TYPE>::from(x); }
 
 // ---- norm --------------------------------------------------------------------
 // Squares and their sums are fp64: a square of a large or small fp32 value leaves fp32's range, and the sum of 10^8 of them its
@@ -168,88 +200,140 @@ __device__ __forceinline__ void norm_chunk(Sum<ORDER>& s, const Chunk<typename E
   }
 }
 
+// Tiles t, t + step, ... below t1 of one tensor.  Those below `keep` are loaded streaming, the others so that they stay in the
+// Infinity Cache (see kKeepBytes).
 template <int ORDER, int TYPE>
-__device__ __forceinline__ void norm_tile(Sum<ORDER>& s, const void* p, int64_t n, int64_t tile) {
+__device__ __forceinline__ void norm_tiles_of(Sum<ORDER>& s, const void* p, int64_t n, int64_t t, int64_t t1, int step, int64_t keep) {
   using Raw = typename Elem<TYPE>::raw;
   constexpr int kPer = 16 / sizeof(Raw);  // elements of a chunk
-  const Raw* g = static_cast<const Raw*>(p);
-  const int64_t first = tile * (kNormTileBytes / sizeof(Raw)), e0 = first + threadIdx.x * kPer;
-  if (first + int64_t(kNormTileBytes / sizeof(Raw)) <= n) {
+  constexpr int64_t kTile = kNormTileBytes / sizeof(Raw);
+  const Raw* at = static_cast<const Raw*>(p) + t * kTile + threadIdx.x * kPer;
+  const int64_t whole = n / kTile < t1 ? n / kTile : t1;
+  // (two loops: of both kinds of load in one the compiler makes plain ones)
+  for (; t < whole && t < keep; t += step, at += step * kTile) {
     Chunk<Raw> c[kNormIters];
 #pragma unroll
-    for (int k = 0; k < kNormIters; k++) c[k] = *reinterpret_cast<const Chunk<Raw>*>(g + e0 + k * kThreads * kPer);
+    for (int k = 0; k < kNormIters; k++) {
+      const Chunk<Raw>* q = reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+#pragma unroll
+      for (int i = 0; i < 4; i++) c[k].w[i] = __builtin_nontemporal_load(&q->w[i]);
+    }
 #pragma unroll
     for (int k = 0; k < kNormIters; k++) norm_chunk<ORDER, TYPE>(s, c[k]);
-    return;
   }
+  for (; t < whole; t += step, at += step * kTile) {
+    Chunk<Raw> c[kNormIters];
 #pragma unroll
-  for (int k = 0; k < kNormIters; k++) {
-    const int64_t e = e0 + k * kThreads * kPer;
-    if (e + kPer <= n) {
-      norm_chunk<ORDER, TYPE>(s, *reinterpret_cast<const Chunk<Raw>*>(g + e));
-    } else {
-      for (int64_t x = e; x < n; x++) s.add(Elem<TYPE>::to(g[x]));
-    }
+    for (int k = 0; k < kNormIters; k++) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+#pragma unroll
+    for (int k = 0; k < kNormIters; k++) norm_chunk<ORDER, TYPE>(s, c[k]);
+  }
+  if (t < t1) {
+    // The tensor's last tile: whole chunks, and what is left of the last one an element to a lane; all requested together.
+    const int64_t left = n - t * kTile;
+    const int chunks = int(left / kPer), rest = int(left % kPer);
+    Chunk<Raw> c[kNormIters];
+    float one = 0.f;
+    if (int(threadIdx.x) < rest) one = load1<TYPE>(p, n - rest + threadIdx.x);
+#pragma unroll
+    for (int k = 0; k < kNormIters; k++)
+      if (k * kThreads + int(threadIdx.x) < chunks) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+#pragma unroll
+    for (int k = 0; k < kNormIters; k++)
+      if (k * kThreads + int(threadIdx.x) < chunks) norm_chunk<ORDER, TYPE>(s, c[k]);
+    s.add(one);
   }
 }
 
-// Over the workgroup, the same order of additions whatever the timing; every lane gets the result of thread 0's wave.
+// Over a workgroup of `waves` waves, the same order of additions whatever the timing; every lane gets the result.
 template <int ORDER>
-__device__ __forceinline__ double block_join(double v, double* lds) {
+__device__ __forceinline__ double block_join(double v, double* lds, int waves) {
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) v = Sum<ORDER>::join(v, __shfl_xor(v, o, kWave));
   if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
   v = lds[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / kWave; w++) v = Sum<ORDER>::join(v, lds[w]);
+  for (int w = 1; w < waves; w++) v = Sum<ORDER>::join(v, lds[w]);
   __syncthreads();
   return v;
 }
 
-// A workgroup sums every gridDim.x-th tile and leaves one partial sum; the last one to arrive joins them in their order, so
-// the result does not depend on who that is.  Lists of more tensors than a table holds take several launches, whose workgroups
-// add to the slots of the one before (the first `valid` of them); only the last joins.
+// The partial sums of all workgroups, in their order.
+template <int ORDER>
+__device__ __forceinline__ double slots_join(const double* slots, int used, double* lds) {
+  double v = 0.0;
+#pragma unroll
+  for (int i = 0; i < kMaxGrid / kThreads; i++)
+    if (i * kThreads + int(threadIdx.x) < used)
+      v = Sum<ORDER>::join(v, __hip_atomic_load(&slots[i * kThreads + threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  return block_join<ORDER>(v, lds, kThreads / kWave);
+}
+
+template <int ORDER>
+__device__ __forceinline__ void norm_result(double* result, double v, int add) {
+  if (add) v = Sum<ORDER>::join(result[0], v);
+  result[0] = v;
+  result[1] = ORDER == 2 ? sqrt(v) : v;
+}
+
+// What a later call reads again should still be in the 256 MB Infinity Cache: the last kKeepBytes of a list are loaded so that they
+// stay there, what lies before them streaming.  302 M bf16 elements (604 MB) clipped into fp32: norm 96 us and clipping 269, with
+// streaming loads throughout 94 and 283, with plain ones 106 and 271.
+constexpr int64_t kKeepBytes = int64_t(192) << 20;
+
+// One pass over the list.  A workgroup sums every gridDim.x-th tile and leaves one partial sum; the last to arrive joins them in
+// their order, so the result does not depend on who that is.  Bound by memory: 604 MB at 6.3 TB/s, 102 MB in 161 tensors 20.5 us (5.0
+// TB/s, of which about 4 us are the launch and the hand-over).  The hand-over is a store, a wait and an atomic of agent scope.
+// Stores of that scope are written through, so the wait for their acknowledgement orders them before the atomic; a release fence,
+// which also writes the L2 cache back, took 45 us more with 2048 workgroups.  Atomics on one address are served about 10 ns apart,
+// hence groups: 102 MB take 28 us with 1024 arrivals at one counter.
+// Lists of more tensors than a table holds take several launches, whose workgroups add to the slots of the one before (the first
+// `valid` of them); only the last joins.
 template <int ORDER, int CAP>
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table<NormSeg, CAP> a, double* result, int valid, int last, int add) {
   __shared__ double lds[kThreads / kWave];
   __shared__ int am_last;
   Sum<ORDER> s;
-  const int tiles = a.tile_start[a.nseg];
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  const int tiles = a.tile_start[a.nseg], step = gridDim.x;
+  const int keep = tiles - int(kKeepBytes / kNormTileBytes);
+  for (int tile = blockIdx.x; tile < tiles;) {
     const int k = find_segment<CAP>(a.tile_start, a.nseg, tile);
     const uint64_t nt = a.seg[k].nt;
-    const int64_t t = tile - a.tile_start[k];
+    const int from = a.tile_start[k], to = a.tile_start[k + 1];
     switch (seg_type(nt)) {
-      case HPX_F32: norm_tile<ORDER, HPX_F32>(s, a.seg[k].g, seg_size(nt), t); break;
-      case HPX_BF16: norm_tile<ORDER, HPX_BF16>(s, a.seg[k].g, seg_size(nt), t); break;
-      default: norm_tile<ORDER, HPX_F16>(s, a.seg[k].g, seg_size(nt), t); break;
+      case HPX_F32: norm_tiles_of<ORDER, HPX_F32>(s, a.seg[k].g, seg_size(nt), tile - from, to - from, step, int64_t(keep) - from); break;
+      case HPX_BF16: norm_tiles_of<ORDER, HPX_BF16>(s, a.seg[k].g, seg_size(nt), tile - from, to - from, step, int64_t(keep) - from); break;
+      default: norm_tiles_of<ORDER, HPX_F16>(s, a.seg[k].g, seg_size(nt), tile - from, to - from, step, int64_t(keep) - from); break;
     }
+    tile += (to - tile + step - 1) / step * step;
   }
-  double v = block_join<ORDER>(s.value(), lds);
+  double v = block_join<ORDER>(s.value(), lds, kThreads / kWave);
+  if (last && gridDim.x == 1 && valid == 0) {
+    if (threadIdx.x == 0) norm_result<ORDER>(result, v, add);
+    return;
+  }
   double* slots = result + kSlots;
   if (threadIdx.x == 0) {
     if (int(blockIdx.x) < valid) v = Sum<ORDER>::join(slots[blockIdx.x], v);
     __hip_atomic_store(&slots[blockIdx.x], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     am_last = 0;
     if (last) {
-      uint32_t* arrivals = reinterpret_cast<uint32_t*>(result + kArrivals);
-      am_last = __hip_atomic_fetch_add(arrivals, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-      if (am_last) __hip_atomic_store(arrivals, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const uint32_t group = blockIdx.x % kGroups, groups = gridDim.x < kGroups ? gridDim.x : kGroups;
+      const uint32_t members = (gridDim.x - group + kGroups - 1) / kGroups;
+      uint32_t* here = reinterpret_cast<uint32_t*>(result + kGroupArrivals + group * kLineDoubles);
+      uint32_t* all = reinterpret_cast<uint32_t*>(result + kArrivals);
+      if (members == 1 || __hip_atomic_fetch_add(here, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == members - 1) {
+        if (members > 1) __hip_atomic_store(here, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        am_last = __hip_atomic_fetch_add(all, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+        if (am_last) __hip_atomic_store(all, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
     }
   }
   __syncthreads();
   if (!am_last) return;
-  const int used = int(gridDim.x) > valid ? int(gridDim.x) : valid;
-  v = 0.0;
-  for (int i = threadIdx.x; i < used; i += kThreads)
-    v = Sum<ORDER>::join(v, __hip_atomic_load(&slots[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  v = block_join<ORDER>(v, lds);
-  if (threadIdx.x == 0) {
-    if (add) v = Sum<ORDER>::join(result[0], v);
-    result[0] = v;
-    result[1] = ORDER == 2 ? sqrt(v) : v;
-  }
+  v = slots_join<ORDER>(slots, int(gridDim.x) > valid ? int(gridDim.x) : valid, lds);
+  if (threadIdx.x == 0) norm_result<ORDER>(result, v, add);
 }
 
 // ---- the coefficient ---------------------------------------------------------
@@ -263,14 +347,16 @@ struct Clip {
 
 // The factor for the gradients, from the sum that a norm call, and perhaps an all-reduce behind it, has left.  A norm that
 // is not finite gives 0, and a factor of 0 means that nothing of the gradient is taken, whatever it holds.
-__device__ __forceinline__ float clip_coefficient(const Clip& a, double* norm) {
-  if (!a.result) return float(a.scale);
-  const double s = a.result[0];
+__device__ __forceinline__ float clip_coefficient(const Clip& a, double s, double* norm) {
   const double n = fabs(a.scale) * (a.order == 2 ? sqrt(s) : s);
   *norm = n;
   if (!(n <= DBL_MAX)) return 0.f;
   const double c = a.max_norm / (n + 1e-6);
   return float(a.scale * (c < 1.0 ? c : 1.0));
+}
+__device__ __forceinline__ float clip_coefficient(const Clip& a, double* norm) {
+  if (!a.result) return float(a.scale);
+  return clip_coefficient(a, a.result[0], norm);
 }
 __device__ __forceinline__ float4 times(float c, float4 g) {
   if (c == 0.f) return make_float4(0.f, 0.f, 0.f, 0.f);
@@ -278,95 +364,254 @@ __device__ __forceinline__ float4 times(float c, float4 g) {
 }
 
 // ---- tiles of the writers ----------------------------------------------------
-// 4096 elements, on boundaries of 4096 elements of the array that is written: a lane's four elements are aligned there.
-constexpr int kIters = 4;
-constexpr int kTileElems = kThreads * 4 * kIters;
+// ITERS x 1024 elements, on boundaries of as many elements of the array that is written: a lane's four elements are aligned there.
+template <int ITERS>
 __host__ __device__ inline int64_t tile_lead(const void* p, int item) {  // elements between the boundary below and p
-  return int64_t((reinterpret_cast<uintptr_t>(p) / item) & (kTileElems - 1));
+  return int64_t((reinterpret_cast<uintptr_t>(p) / item) & (kThreads * 4 * ITERS - 1));
 }
-inline int64_t write_tiles(const void* p, int64_t n, int item) { return (tile_lead(p, item) + n + kTileElems - 1) / kTileElems; }
+template <int ITERS>
+inline int64_t write_tiles(const void* p, int64_t n, int item) { return (tile_lead<ITERS>(p, item) + n + kThreads * 4 * ITERS - 1) / (kThreads * 4 * ITERS); }
 
-// Calls whole(e) for each of the lane's groups of four elements e ... e + 3 that lies in the tensor, one(e) for single ones at
-// the ends.
-template <typename Whole, typename One>
-__device__ __forceinline__ void for_tile(const void* p, int item, int64_t n, int64_t tile, Whole whole, One one) {
-  const int64_t e0 = tile * kTileElems - tile_lead(p, item) + threadIdx.x * 4;
-#pragma unroll
-  for (int k = 0; k < kIters; k++) {
-    const int64_t e = e0 + k * kThreads * 4;
-    if (e >= 0 && e + 4 <= n) {
-      whole(e);
-    } else {
-      for (int64_t x = e; x < e + 4; x++)
-        if (x >= 0 && x < n) one(x);
+// The lane's part of a tile: groups of four elements k * 1024 behind e0, those of them that has(k), and at the tensor's ends, where
+// less than a group is left before the first or behind the last, an element of its own (one >= 0).
+template <int ITERS>
+struct Part {
+  int64_t e0, one;
+  int64_t n;
+  bool whole;
+  __device__ Part(const void* p, int item, int64_t size, int64_t tile) : n(size) {
+    constexpr int64_t kTile = kThreads * 4 * ITERS;
+    const int64_t lead = tile_lead<ITERS>(p, item), first = tile * kTile - lead;
+    e0 = first + threadIdx.x * 4;
+    whole = first >= 0 && first + kTile <= n;
+    one = -1;
+    if (!whole) {
+      const int64_t to_group = (4 - (lead & 3)) & 3, head = to_group < n ? to_group : n, tail = (n - head) & 3;
+      if (first <= 0 && threadIdx.x < head) one = threadIdx.x;
+      if (threadIdx.x >= kWave && threadIdx.x < kWave + tail && n - tail >= first && n - tail < first + kTile) one = n - tail + (threadIdx.x - kWave);
     }
   }
-}
+  __device__ int64_t at(int k) const { return e0 + k * kThreads * 4; }
+  __device__ bool has(int k) const { return whole || (at(k) >= 0 && at(k) + 4 <= n); }
+};
 
-template <int TYPE, int OUT>
-__device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t tile, float c) {
-  using G = typename Elem<TYPE>::raw;
-  using O = typename Elem<OUT>::raw;
-  for_tile(
-      sg.out, sizeof(O), n, tile, [&](int64_t e) { store4<OUT>(sg.out, e, times(c, load4<TYPE>(sg.g, e))); },
-      [&](int64_t e) {
-        const float g = Elem<TYPE>::to(static_cast<const G*>(sg.g)[e]);
-        static_cast<O*>(sg.out)[e] = Elem<OUT>::from(c == 0.f ? 0.f : c * g);
-      });
-}
-
-template <int CAP>
-__global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result) {
-  const int tile = blockIdx.x;
-  double norm = 0.0;
-  const float c = clip_coefficient(clip, &norm);
-  if (clip.tell && tile == 0 && threadIdx.x == 0) {
-    result[1] = norm;
-    result[2] = double(c);
+// The gradient is requested first; coefficient() is called by every lane of the workgroup.
+constexpr int kClipIters = 2;
+template <int TYPE, int OUT, typename Coefficient>
+__device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t tile, Coefficient coefficient) {
+  const Part<kClipIters> part(sg.out, sizeof(typename Elem<OUT>::raw), n, tile);
+  raw4<TYPE> g[kClipIters];
+  if (part.whole) {
+#pragma unroll
+    for (int k = 0; k < kClipIters; k++) g[k] = load4_stream<TYPE>(sg.g, part.at(k));
+    const float c = coefficient();
+#pragma unroll
+    for (int k = 0; k < kClipIters; k++) store4_stream<OUT>(sg.out, part.at(k), times(c, value4<TYPE>(g[k])));
+    return;
   }
+  float one = 0.f;
+  if (part.one >= 0) one = load1<TYPE>(sg.g, part.one);
+#pragma unroll
+  for (int k = 0; k < kClipIters; k++)
+    if (part.has(k)) g[k] = load4<TYPE>(sg.g, part.at(k));
+  const float c = coefficient();
+#pragma unroll
+  for (int k = 0; k < kClipIters; k++)
+    if (part.has(k)) store4_stream<OUT>(sg.out, part.at(k), times(c, value4<TYPE>(g[k])));
+  if (part.one >= 0) store1<OUT>(sg.out, part.one, c == 0.f ? 0.f : c * one);
+}
+
+// Second pass of a clipping call.  With `slots` the pass before has left its partial sums and nobody has joined them: every
+// workgroup does that for itself while its gradients are on the way, which saves the hand-over at the end of that pass and costs a
+// walk over the slots in each: 3 M elements (1500 tiles) 10.5 us against 11.9 and 12.5 against 14.2, 6 M (2900 tiles) 14.8 against
+// 16.3, 10 M (4900 tiles) 26.0 against 25.7.
+// Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 29.5 us (6.9 TB/s read and written), 110 M of a mixed
+// list 91.8 (7.2 TB/s).
+constexpr int64_t kJoinTiles = 4096;
+template <int ORDER, int CAP>
+__global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result, int slots) {
+  __shared__ double lds[kThreads / kWave];
+  const int tile = blockIdx.x;
+  auto coefficient = [&]() -> float {
+    const double s = slots ? slots_join<ORDER>(result + kSlots, slots, lds) : result[0];
+    double norm = 0.0;
+    const float c = clip_coefficient(clip, s, &norm);
+    if (clip.tell && tile == 0 && threadIdx.x == 0) {
+      if (slots) result[0] = s;
+      result[1] = norm;
+      result[2] = double(c);
+    }
+    return c;
+  };
   const int k = find_segment<CAP>(a.tile_start, a.nseg, tile);
   const ClipSeg sg = a.seg[k];
   const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
-  if (n == 0) return;
-  if (sg.out == sg.g) {
-    if (c == 1.f) return;
+  if (sg.out == sg.g) {  // in place, or nothing at all
+    const float c = coefficient();
+    if (c == 1.f || n == 0) return;
+    auto known = [c]() { return c; };
     switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, c); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16>(sg, n, t, c); break;
-      default: clip_tile<HPX_F16, HPX_F16>(sg, n, t, c); break;
+      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, known); break;
+      case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16>(sg, n, t, known); break;
+      default: clip_tile<HPX_F16, HPX_F16>(sg, n, t, known); break;
     }
   } else {
     switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, c); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_F32>(sg, n, t, c); break;
-      default: clip_tile<HPX_F16, HPX_F32>(sg, n, t, c); break;
+      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, coefficient); break;
+      case HPX_BF16: clip_tile<HPX_BF16, HPX_F32>(sg, n, t, coefficient); break;
+      default: clip_tile<HPX_F16, HPX_F32>(sg, n, t, coefficient); break;
+    }
+  }
+}
+
+// A short list in one launch of one workgroup, which keeps it in registers between the norm and the product: a wave takes 1024
+// elements of one tensor at a time, three times at most.  One CU moves some 100 GB/s, so what the second launch costs is the limit:
+// 8 thousand elements 4.5 us against 7.9 in two launches, 33 thousand 6.2 against 7.9, 60 thousand (in four rounds) 8.0 against 7.9.
+constexpr int kShortThreads = 1024;
+constexpr int kShortTile = kWave * 16;
+constexpr int kShortRounds = 3;
+constexpr int kShortTiles = kShortRounds * kShortThreads / kWave;  // 48, so at most as many tensors
+static_assert(kShortTiles <= kWave, "the table is read by one wave");
+
+struct ShortPart {  // the lane's elements of a tile: four groups of four, and one of those behind the last whole group
+  float4 v[4];
+  float one;
+};
+template <int TYPE>
+__device__ __forceinline__ void short_load(ShortPart& p, const void* g, int64_t n, int64_t first) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t rest = n & 3, e0 = first + lane * 4;
+  raw4<TYPE> r[4];
+  p.one = n - rest < first + kShortTile && lane < rest ? load1<TYPE>(g, n - rest + lane) : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int64_t e = e0 + k * kWave * 4;
+    if (e + 4 <= n) r[k] = load4<TYPE>(g, e);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) p.v[k] = e0 + k * kWave * 4 + 4 <= n ? value4<TYPE>(r[k]) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+template <int OUT>
+__device__ __forceinline__ void short_store(const ShortPart& p, void* out, int64_t n, int64_t first, float c) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t rest = n & 3, e0 = first + lane * 4;
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (e0 + k * kWave * 4 + 4 <= n) store4_stream<OUT>(out, e0 + k * kWave * 4, times(c, p.v[k]));
+  if (n - rest < first + kShortTile && lane < rest) store1<OUT>(out, n - rest + lane, c == 0.f ? 0.f : c * p.one);
+}
+
+template <int ORDER>
+__global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Table<ClipSeg, kShortTiles> a, const Clip clip, double* result) {
+  __shared__ double lds[kShortThreads / kWave];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), tiles = a.tile_start[a.nseg];
+  ShortPart part[kShortRounds];
+  int seg[kShortRounds];
+  Sum<ORDER> s;
+#pragma unroll
+  for (int r = 0; r < kShortRounds; r++) {
+    const int tile = r * (kShortThreads / kWave) + wave;
+    if (tile < tiles) {
+      const int k = __builtin_amdgcn_readfirstlane(find_segment<kShortTiles>(a.tile_start, a.nseg, tile));
+      const uint64_t nt = a.seg[k].nt;
+      const int64_t n = seg_size(nt), first = int64_t(tile - a.tile_start[k]) * kShortTile;
+      seg[r] = k;
+      switch (seg_type(nt)) {
+        case HPX_F32: short_load<HPX_F32>(part[r], a.seg[k].g, n, first); break;
+        case HPX_BF16: short_load<HPX_BF16>(part[r], a.seg[k].g, n, first); break;
+        default: short_load<HPX_F16>(part[r], a.seg[k].g, n, first); break;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kShortRounds; r++)
+    if (r * (kShortThreads / kWave) + wave < tiles) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) { s.add(part[r].v[k].x); s.add(part[r].v[k].y); s.add(part[r].v[k].z); s.add(part[r].v[k].w); }
+      s.add(part[r].one);
+    }
+  const double sum = block_join<ORDER>(s.value(), lds, kShortThreads / kWave);
+  double norm = 0.0;
+  const float c = clip_coefficient(clip, sum, &norm);
+  if (threadIdx.x == 0) {
+    result[0] = sum;
+    result[1] = norm;
+    result[2] = double(c);
+  }
+#pragma unroll
+  for (int r = 0; r < kShortRounds; r++) {
+    const int tile = r * (kShortThreads / kWave) + wave;
+    if (tile < tiles) {
+      const int k = seg[r];
+      const ClipSeg sg = a.seg[k];
+      const int64_t n = seg_size(sg.nt), first = int64_t(tile - a.tile_start[k]) * kShortTile;
+      const int out = sg.out == sg.g ? seg_type(sg.nt) : HPX_F32;
+      if (sg.out == sg.g && c == 1.f) continue;
+      switch (out) {
+        case HPX_F32: short_store<HPX_F32>(part[r], sg.out, n, first, c); break;
+        case HPX_BF16: short_store<HPX_BF16>(part[r], sg.out, n, first, c); break;
+        default: short_store<HPX_F16>(part[r], sg.out, n, first, c); break;
+      }
     }
   }
 }
 
 // ---- momentum ----------------------------------------------------------------
 // u' = m u + c g with the product c g rounded once and one rounding for the rest (fma), d = m u' + c g likewise.
-template <int TYPE>
+__device__ __forceinline__ float4 axpy(float m, float4 x, float4 y) { return make_float4(fmaf(m, x.x, y.x), fmaf(m, x.y, y.y), fmaf(m, x.z, y.z), fmaf(m, x.w, y.w)); }
+
+// Tiles of 4096 elements; with a direction to write as well, tiles of 2048.  Bound by memory: 138 M fp32 elements 258 us (6.4 TB/s; 275
+// with tiles of 2048), 100 M 183 (196); with a direction, 100 M bf16 elements 225 us (6.2 TB/s; 243 with tiles of 4096), 25.6 M in
+// 161 tensors 58.7 (61.7).  Launches ask for LDS they do not touch, so that a CU holds three workgroups (see kWriteStreamPadLds3): 302 M
+// bf16 elements 463 us, 478 with four, 484 with eight.
+template <bool DIRECTION>
+constexpr int kMomentumIters = DIRECTION ? 2 : 4;
+template <int TYPE, bool DIRECTION>
 __device__ __forceinline__ void momentum_tile(const MomentumSeg& sg, int64_t n, int64_t tile, float m, float c) {
-  using G = typename Elem<TYPE>::raw;
-  for_tile(
-      sg.u, 4, n, tile,
-      [&](int64_t e) {
-        const float4 g = times(c, load4<TYPE>(sg.g, e));
-        float4 u = ld4(sg.u + e);
-        u = make_float4(fmaf(m, u.x, g.x), fmaf(m, u.y, g.y), fmaf(m, u.z, g.z), fmaf(m, u.w, g.w));
-        st4(sg.u + e, u);
-        if (sg.d) st4(sg.d + e, make_float4(fmaf(m, u.x, g.x), fmaf(m, u.y, g.y), fmaf(m, u.z, g.z), fmaf(m, u.w, g.w)));
-      },
-      [&](int64_t e) {
-        const float g = c == 0.f ? 0.f : c * Elem<TYPE>::to(static_cast<const G*>(sg.g)[e]);
-        const float u = fmaf(m, sg.u[e], g);
-        sg.u[e] = u;
-        if (sg.d) sg.d[e] = fmaf(m, u, g);
-      });
+  constexpr int kIters = kMomentumIters<DIRECTION>;
+  const Part<kIters> part(sg.u, 4, n, tile);
+  raw4<TYPE> g[kIters];
+  raw4<HPX_F32> u[kIters];
+  if (part.whole) {
+#pragma unroll
+    for (int k = 0; k < kIters; k++) {
+      g[k] = load4_stream<TYPE>(sg.g, part.at(k));
+      u[k] = load4_stream<HPX_F32>(sg.u, part.at(k));
+    }
+#pragma unroll
+    for (int k = 0; k < kIters; k++) {
+      const float4 cg = times(c, value4<TYPE>(g[k])), v = axpy(m, value4<HPX_F32>(u[k]), cg);
+      store4_stream<HPX_F32>(sg.u, part.at(k), v);
+      if (DIRECTION) store4_stream<HPX_F32>(sg.d, part.at(k), axpy(m, v, cg));
+    }
+    return;
+  }
+  float g1 = 0.f, u1 = 0.f;
+  if (part.one >= 0) {
+    g1 = load1<TYPE>(sg.g, part.one);
+    u1 = sg.u[part.one];
+  }
+#pragma unroll
+  for (int k = 0; k < kIters; k++)
+    if (part.has(k)) {
+      g[k] = load4<TYPE>(sg.g, part.at(k));
+      u[k] = load4<HPX_F32>(sg.u, part.at(k));
+    }
+#pragma unroll
+  for (int k = 0; k < kIters; k++)
+    if (part.has(k)) {
+      const float4 cg = times(c, value4<TYPE>(g[k])), v = axpy(m, value4<HPX_F32>(u[k]), cg);
+      store4_stream<HPX_F32>(sg.u, part.at(k), v);
+      if (DIRECTION) store4_stream<HPX_F32>(sg.d, part.at(k), axpy(m, v, cg));
+    }
+  if (part.one >= 0) {
+    const float cg = c == 0.f ? 0.f : c * g1, v = fmaf(m, u1, cg);
+    sg.u[part.one] = v;
+    if (DIRECTION) sg.d[part.one] = fmaf(m, v, cg);
+  }
 }
 
-template <int CAP>
+template <bool DIRECTION, int CAP>
 __global__ __launch_bounds__(kThreads) void gd_momentum_kernel(const Table<MomentumSeg, CAP> a, const Clip clip, double* result, float m) {
   const int tile = blockIdx.x;
   double norm = 0.0;
@@ -380,9 +625,9 @@ __global__ __launch_bounds__(kThreads) void gd_momentum_kernel(const Table<Momen
   const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
   if (n == 0) return;
   switch (seg_type(sg.nt)) {
-    case HPX_F32: momentum_tile<HPX_F32>(sg, n, t, m, c); break;
-    case HPX_BF16: momentum_tile<HPX_BF16>(sg, n, t, m, c); break;
-    default: momentum_tile<HPX_F16>(sg, n, t, m, c); break;
+    case HPX_F32: momentum_tile<HPX_F32, DIRECTION>(sg, n, t, m, c); break;
+    case HPX_BF16: momentum_tile<HPX_BF16, DIRECTION>(sg, n, t, m, c); break;
+    default: momentum_tile<HPX_F16, DIRECTION>(sg, n, t, m, c); break;
   }
 }
 
@@ -473,10 +718,11 @@ int for_tables(int count, Fill fill, Launch launch) {
   return HPX_OK;
 }
 
+// slots: not null where the caller joins the partial sums itself; gets their number.
 template <int ORDER, int CAP>
-int launch_norm(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, int add, double* result, hipStream_t st) {
+int launch_norm(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, int add, double* result, int* slots, hipStream_t st) {
   int valid = 0;
-  return for_tables<NormSeg, CAP>(
+  const int rc = for_tables<NormSeg, CAP>(
       count,
       [&](int i, NormSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
@@ -486,29 +732,31 @@ int launch_norm(int count, const void* const* grads, const int64_t* sizes, const
       },
       [&](const Table<NormSeg, CAP>& a, int tiles, bool last) -> int {
         const int grid = std::max(1, std::min(tiles, kMaxGrid));
-        HPX_LAUNCH("grad_norm_kernel", (grad_norm_kernel<ORDER, CAP>), dim3(grid), dim3(kThreads), st, a, result, valid, int(last), add);
+        HPX_LAUNCH("grad_norm_kernel", (grad_norm_kernel<ORDER, CAP>), dim3(grid), dim3(kThreads), st, a, result, valid, int(last && !slots), add);
         HPX_HIP(hipGetLastError());
         valid = std::max(valid, grid);
         return HPX_OK;
       });
+  if (slots) *slots = valid;
+  return rc;
 }
-int norm(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, int order, int add, double* result, hipStream_t st) {
-  if (order == 2)
-    return count <= kCapSmall ? launch_norm<2, kCapSmall>(count, grads, sizes, types, add, result, st)
-                              : launch_norm<2, NormSeg::kCapLarge>(count, grads, sizes, types, add, result, st);
-  return count <= kCapSmall ? launch_norm<HPX_NORM_MAX, kCapSmall>(count, grads, sizes, types, add, result, st)
-                            : launch_norm<HPX_NORM_MAX, NormSeg::kCapLarge>(count, grads, sizes, types, add, result, st);
+template <int ORDER>
+int norm(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, int add, double* result, int* slots, hipStream_t st) {
+  return count <= kCapSmall ? launch_norm<ORDER, kCapSmall>(count, grads, sizes, types, add, result, slots, st)
+                            : launch_norm<ORDER, NormSeg::kCapLarge>(count, grads, sizes, types, add, result, slots, st);
 }
 
-template <int CAP>
-int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, Clip clip, double* result, hipStream_t st) {
+ClipSeg clip_seg(const void* g, void* out, int64_t size, int type) { return ClipSeg{g, out, uint64_t(size) | uint64_t(type) << kTypeShift}; }
+
+template <int ORDER, int CAP>
+int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, Clip clip, double* result, int slots, hipStream_t st) {
   return for_tables<ClipSeg, CAP>(
       count,
       [&](int i, ClipSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
-        sg = ClipSeg{grads[i], outs[i], uint64_t(sizes[i]) | uint64_t(type) << kTypeShift};
-        return write_tiles(outs[i], sizes[i], outs[i] == grads[i] ? item_size(type) : 4);
+        sg = clip_seg(grads[i], outs[i], sizes[i], type);
+        return write_tiles<kClipIters>(outs[i], sizes[i], outs[i] == grads[i] ? item_size(type) : 4);
       },
       [&](Table<ClipSeg, CAP>& a, int tiles, bool) -> int {
         if (tiles == 0) {  // norm and coefficient are told all the same
@@ -518,14 +766,46 @@ int launch_clip(int count, const void* const* grads, const int64_t* sizes, const
           a.tile_start[1] = 1;
           tiles = 1;
         }
-        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result);
+        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<ORDER, CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result, slots);
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
       });
 }
 
-template <int CAP>
+// Lists of up to kShortTiles tiles of 1024 elements: one launch of one workgroup.
+template <int ORDER>
+int launch_clip_short(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, const Clip& clip, double* result, hipStream_t st) {
+  return for_tables<ClipSeg, kShortTiles>(
+      count,
+      [&](int i, ClipSeg& sg) -> int64_t {
+        sg = clip_seg(grads[i], outs[i], sizes[i], types ? types[i] : HPX_F32);
+        return (sizes[i] + kShortTile - 1) / kShortTile;
+      },
+      [&](const Table<ClipSeg, kShortTiles>& a, int, bool) -> int {
+        HPX_LAUNCH("grad_clip_short_kernel", (grad_clip_short_kernel<ORDER>), dim3(1), dim3(kShortThreads), st, a, clip, result);
+        HPX_HIP(hipGetLastError());
+        return HPX_OK;
+      });
+}
+
+template <int ORDER>
+int clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, bool measured, const Clip& clip, double* result, hipStream_t st) {
+  int slots = 0;
+  if (!measured) {
+    int64_t short_tiles = 0, tiles = 0;
+    for (int i = 0; i < count; i++) {
+      short_tiles += (sizes[i] + kShortTile - 1) / kShortTile;
+      tiles += sizes[i] ? (sizes[i] + 2 * kThreads * 4 * kClipIters - 2) / (kThreads * 4 * kClipIters) : 0;  // at most
+    }
+    if (short_tiles <= kShortTiles) return launch_clip_short<ORDER>(count, grads, sizes, types, outs, clip, result, st);
+    if (const int rc = norm<ORDER>(count, grads, sizes, types, 0, result, tiles <= kJoinTiles ? &slots : nullptr, st)) return rc;
+  }
+  if (count <= kCapSmall) return launch_clip<ORDER, kCapSmall>(count, grads, sizes, types, outs, clip, result, slots, st);
+  return launch_clip<ORDER, ClipSeg::kCapLarge>(count, grads, sizes, types, outs, clip, result, slots, st);
+}
+
+template <bool DIRECTION, int CAP>
 int launch_momentum(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, float* const* us, float* const* outs, float m, Clip clip, double* result,
                     hipStream_t st) {
   return for_tables<MomentumSeg, CAP>(
@@ -534,7 +814,7 @@ int launch_momentum(int count, const void* const* grads, const int64_t* sizes, c
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
         sg = MomentumSeg{grads[i], us[i], outs ? outs[i] : nullptr, uint64_t(sizes[i]) | uint64_t(type) << kTypeShift};
-        return write_tiles(us[i], sizes[i], 4);
+        return write_tiles<kMomentumIters<DIRECTION>>(us[i], sizes[i], 4);
       },
       [&](Table<MomentumSeg, CAP>& a, int tiles, bool) -> int {
         if (tiles == 0) {
@@ -544,7 +824,7 @@ int launch_momentum(int count, const void* const* grads, const int64_t* sizes, c
           a.tile_start[1] = 1;
           tiles = 1;
         }
-        HPX_LAUNCH("gd_momentum_kernel", (gd_momentum_kernel<CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result, m);
+        HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, CAP>), dim3(tiles), dim3(kThreads), kWriteStreamPadLds3, st, a, clip, result, m);
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
@@ -620,7 +900,9 @@ HPX_API int hpx_grad_norm(int count, const void* const* grads, const int64_t* si
     if (const int rc = check_clip(who, order, 0.0, 1.0)) return rc;
     if (const int rc = check_result(who, result)) return rc;
     if (const int rc = check_list(who, count, grads, sizes, types)) return rc;
-    return norm(count, grads, sizes, types, order, is_add_to != 0, result, static_cast<hipStream_t>(stream));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return order == 2 ? norm<2>(count, grads, sizes, types, is_add_to != 0, result, nullptr, st)
+                      : norm<HPX_NORM_MAX>(count, grads, sizes, types, is_add_to != 0, result, nullptr, st);
   });
 }
 
@@ -641,11 +923,9 @@ HPX_API int hpx_grad_clip(int count, const void* const* grads, const int64_t* si
     }
     if (const int rc = check_writes(who, count, grads, sizes, types, to.data(), nullptr, to.data())) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!is_measured)
-      if (const int rc = norm(count, grads, sizes, types, order, 0, result, st)) return rc;
-    const Clip clip{result, max_norm, scale, order, 1};
-    if (count <= kCapSmall) return launch_clip<kCapSmall>(count, grads, sizes, types, to.data(), clip, result, st);
-    return launch_clip<ClipSeg::kCapLarge>(count, grads, sizes, types, to.data(), clip, result, st);
+    const Clip how{result, max_norm, scale, order, 1};
+    return order == 2 ? clip<2>(count, grads, sizes, types, to.data(), is_measured != 0, how, result, st)
+                      : clip<HPX_NORM_MAX>(count, grads, sizes, types, to.data(), is_measured != 0, how, result, st);
   });
 }
 
@@ -669,8 +949,12 @@ HPX_API int hpx_gd_momentum(int count, const void* const* grads, const int64_t* 
     if (const int rc = check_writes(who, count, grads, sizes, types, reinterpret_cast<const void* const*>(momenta), ds, ds)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Clip clip{result, max_norm, scale, order, result != nullptr};
-    if (count <= kCapSmall) return launch_momentum<kCapSmall>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
-    return launch_momentum<MomentumSeg::kCapLarge>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
+    auto launch = [&](auto direction) -> int {
+      constexpr bool D = decltype(direction)::value;
+      if (count <= kCapSmall) return launch_momentum<D, kCapSmall>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
+      return launch_momentum<D, MomentumSeg::kCapLarge>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
+    };
+    return outs ? launch(std::true_type{}) : launch(std::false_type{});
   });
 }
 
