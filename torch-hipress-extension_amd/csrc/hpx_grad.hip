@@ -109,20 +109,21 @@ struct __attribute__((packed, aligned(sizeof(Raw)))) Raw4 {
 template <int TYPE>
 using raw4 = Raw4<typename Elem<TYPE>::raw>;
 
-template <int TYPE>
+// STREAM: with the non-temporal hint (see ld4_stream), which a list larger than kPlainBytes wants; one that is smaller may lie in the
+// caches, and stays there.
+template <int TYPE, bool STREAM>
 __device__ __forceinline__ raw4<TYPE> load4(const void* base, int64_t e) {
-  return *reinterpret_cast<const raw4<TYPE>*>(static_cast<const typename Elem<TYPE>::raw*>(base) + e);
-}
-// Streaming forms (see ld4_stream): 138 M elements of momentum correction take 258 us with both, 297 with plain loads, 300 with
-// plain loads and stores.
-template <int TYPE>
-__device__ __forceinline__ raw4<TYPE> load4_stream(const void* base, int64_t e) {
   const raw4<TYPE>* q = reinterpret_cast<const raw4<TYPE>*>(static_cast<const typename Elem<TYPE>::raw*>(base) + e);
+  if constexpr (!STREAM) return *q;
   raw4<TYPE> r;
 #pragma unroll
   for (unsigned i = 0; i < sizeof(typename Elem<TYPE>::raw); i++) r.w[i] = __builtin_nontemporal_load(&q->w[i]);
   return r;
 }
+// Bytes that a writing pass reads.  Plain / streaming loads: clipping 16 M fp32 elements 33.0 / 34.2 us, 32 M 61.4 / 60.4, 64 M bf16
+// 79.6 / 78.6; momentum of 4 M fp32 elements 9.5 / 10.1, 12 M (96 MB) 24.1 / 24.8, 16 M 34.8 / 31.7, 138 M 297 / 258.  Stores stream at
+// every size: clipping 4 M elements 13.0 us against 14.1 with plain ones, 64 M 117 against 139.
+constexpr int64_t kPlainBytes = int64_t(96) << 20;
 template <int TYPE>
 __device__ __forceinline__ void store4_stream(void* base, int64_t e, float4 x) {
   using E = Elem<TYPE>;
@@ -397,13 +398,13 @@ struct Part {
 
 // The gradient is requested first; coefficient() is called by every lane of the workgroup.
 constexpr int kClipIters = 2;
-template <int TYPE, int OUT, typename Coefficient>
+template <int TYPE, int OUT, bool STREAM, typename Coefficient>
 __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t tile, Coefficient coefficient) {
   const Part<kClipIters> part(sg.out, sizeof(typename Elem<OUT>::raw), n, tile);
   raw4<TYPE> g[kClipIters];
   if (part.whole) {
 #pragma unroll
-    for (int k = 0; k < kClipIters; k++) g[k] = load4_stream<TYPE>(sg.g, part.at(k));
+    for (int k = 0; k < kClipIters; k++) g[k] = load4<TYPE, STREAM>(sg.g, part.at(k));
     const float c = coefficient();
 #pragma unroll
     for (int k = 0; k < kClipIters; k++) store4_stream<OUT>(sg.out, part.at(k), times(c, value4<TYPE>(g[k])));
@@ -413,7 +414,7 @@ __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t 
   if (part.one >= 0) one = load1<TYPE>(sg.g, part.one);
 #pragma unroll
   for (int k = 0; k < kClipIters; k++)
-    if (part.has(k)) g[k] = load4<TYPE>(sg.g, part.at(k));
+    if (part.has(k)) g[k] = load4<TYPE, STREAM>(sg.g, part.at(k));
   const float c = coefficient();
 #pragma unroll
   for (int k = 0; k < kClipIters; k++)
@@ -428,7 +429,7 @@ __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t 
 // Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 29.5 us (6.9 TB/s read and written), 110 M of a mixed
 // list 91.8 (7.2 TB/s).
 constexpr int64_t kJoinTiles = 4096;
-template <int ORDER, int CAP>
+template <int ORDER, bool STREAM, int CAP>
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result, int slots) {
   __shared__ double lds[kThreads / kWave];
   const int tile = blockIdx.x;
@@ -451,15 +452,15 @@ __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg
     if (c == 1.f || n == 0) return;
     auto known = [c]() { return c; };
     switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, known); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16>(sg, n, t, known); break;
-      default: clip_tile<HPX_F16, HPX_F16>(sg, n, t, known); break;
+      case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, known); break;
+      case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16, STREAM>(sg, n, t, known); break;
+      default: clip_tile<HPX_F16, HPX_F16, STREAM>(sg, n, t, known); break;
     }
   } else {
     switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32>(sg, n, t, coefficient); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_F32>(sg, n, t, coefficient); break;
-      default: clip_tile<HPX_F16, HPX_F32>(sg, n, t, coefficient); break;
+      case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, coefficient); break;
+      case HPX_BF16: clip_tile<HPX_BF16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
+      default: clip_tile<HPX_F16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
     }
   }
 }
@@ -486,7 +487,7 @@ __device__ __forceinline__ void short_load(ShortPart& p, const void* g, int64_t 
 #pragma unroll
   for (int k = 0; k < 4; k++) {
     const int64_t e = e0 + k * kWave * 4;
-    if (e + 4 <= n) r[k] = load4<TYPE>(g, e);
+    if (e + 4 <= n) r[k] = load4<TYPE, false>(g, e);
   }
 #pragma unroll
   for (int k = 0; k < 4; k++) p.v[k] = e0 + k * kWave * 4 + 4 <= n ? value4<TYPE>(r[k]) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -562,11 +563,12 @@ __device__ __forceinline__ float4 axpy(float m, float4 x, float4 y) { return mak
 
 // Tiles of 4096 elements; with a direction to write as well, tiles of 2048.  Bound by memory: 138 M fp32 elements 258 us (6.4 TB/s; 275
 // with tiles of 2048), 100 M 183 (196); with a direction, 100 M bf16 elements 225 us (6.2 TB/s; 243 with tiles of 4096), 25.6 M in
-// 161 tensors 58.7 (61.7).  Launches ask for LDS they do not touch, so that a CU holds three workgroups (see kWriteStreamPadLds3): 302 M
-// bf16 elements 463 us, 478 with four, 484 with eight.
+// 161 tensors 58.7 (61.7).  Streaming launches ask for LDS they do not touch, so that a CU holds three workgroups (see
+// kWriteStreamPadLds3): 302 M bf16 elements 463 us, 477 with four, 482 with eight; 130 M in 100 tensors 202, 206, 207; one fp32 tensor of
+// 25 M 49.0, 47.7, 47.6.
 template <bool DIRECTION>
 constexpr int kMomentumIters = DIRECTION ? 2 : 4;
-template <int TYPE, bool DIRECTION>
+template <int TYPE, bool DIRECTION, bool STREAM>
 __device__ __forceinline__ void momentum_tile(const MomentumSeg& sg, int64_t n, int64_t tile, float m, float c) {
   constexpr int kIters = kMomentumIters<DIRECTION>;
   const Part<kIters> part(sg.u, 4, n, tile);
@@ -575,8 +577,8 @@ __device__ __forceinline__ void momentum_tile(const MomentumSeg& sg, int64_t n, 
   if (part.whole) {
 #pragma unroll
     for (int k = 0; k < kIters; k++) {
-      g[k] = load4_stream<TYPE>(sg.g, part.at(k));
-      u[k] = load4_stream<HPX_F32>(sg.u, part.at(k));
+      g[k] = load4<TYPE, STREAM>(sg.g, part.at(k));
+      u[k] = load4<HPX_F32, STREAM>(sg.u, part.at(k));
     }
 #pragma unroll
     for (int k = 0; k < kIters; k++) {
@@ -594,8 +596,8 @@ __device__ __forceinline__ void momentum_tile(const MomentumSeg& sg, int64_t n, 
 #pragma unroll
   for (int k = 0; k < kIters; k++)
     if (part.has(k)) {
-      g[k] = load4<TYPE>(sg.g, part.at(k));
-      u[k] = load4<HPX_F32>(sg.u, part.at(k));
+      g[k] = load4<TYPE, STREAM>(sg.g, part.at(k));
+      u[k] = load4<HPX_F32, STREAM>(sg.u, part.at(k));
     }
 #pragma unroll
   for (int k = 0; k < kIters; k++)
@@ -611,7 +613,7 @@ __device__ __forceinline__ void momentum_tile(const MomentumSeg& sg, int64_t n, 
   }
 }
 
-template <bool DIRECTION, int CAP>
+template <bool DIRECTION, bool STREAM, int CAP>
 __global__ __launch_bounds__(kThreads) void gd_momentum_kernel(const Table<MomentumSeg, CAP> a, const Clip clip, double* result, float m) {
   const int tile = blockIdx.x;
   double norm = 0.0;
@@ -625,9 +627,9 @@ __global__ __launch_bounds__(kThreads) void gd_momentum_kernel(const Table<Momen
   const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
   if (n == 0) return;
   switch (seg_type(sg.nt)) {
-    case HPX_F32: momentum_tile<HPX_F32, DIRECTION>(sg, n, t, m, c); break;
-    case HPX_BF16: momentum_tile<HPX_BF16, DIRECTION>(sg, n, t, m, c); break;
-    default: momentum_tile<HPX_F16, DIRECTION>(sg, n, t, m, c); break;
+    case HPX_F32: momentum_tile<HPX_F32, DIRECTION, STREAM>(sg, n, t, m, c); break;
+    case HPX_BF16: momentum_tile<HPX_BF16, DIRECTION, STREAM>(sg, n, t, m, c); break;
+    default: momentum_tile<HPX_F16, DIRECTION, STREAM>(sg, n, t, m, c); break;
   }
 }
 
@@ -656,6 +658,18 @@ __global__ __launch_bounds__(kThreads) void gd_mask_kernel(const Table<MaskSeg, 
 // ---- host --------------------------------------------------------------------
 int item_size(int type) { return type == HPX_F32 ? 4 : 2; }
 bool aligned(const void* p, int item) { return reinterpret_cast<uintptr_t>(p) % item == 0; }
+
+int64_t list_bytes(int count, const int64_t* sizes, const int32_t* types) {
+  int64_t b = 0;
+  for (int i = 0; i < count; i++) b += sizes[i] * item_size(types ? types[i] : HPX_F32);
+  return b;
+}
+// f with two truth values as types.
+template <typename F>
+int with_constants(bool a, bool b, F f) {
+  if (a) return b ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+  return b ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+}
 
 struct Span {
   uintptr_t b, e;
@@ -748,7 +762,7 @@ int norm(int count, const void* const* grads, const int64_t* sizes, const int32_
 
 ClipSeg clip_seg(const void* g, void* out, int64_t size, int type) { return ClipSeg{g, out, uint64_t(size) | uint64_t(type) << kTypeShift}; }
 
-template <int ORDER, int CAP>
+template <int ORDER, bool STREAM, int CAP>
 int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, Clip clip, double* result, int slots, hipStream_t st) {
   return for_tables<ClipSeg, CAP>(
       count,
@@ -766,7 +780,7 @@ int launch_clip(int count, const void* const* grads, const int64_t* sizes, const
           a.tile_start[1] = 1;
           tiles = 1;
         }
-        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<ORDER, CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result, slots);
+        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<ORDER, STREAM, CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result, slots);
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
@@ -801,11 +815,13 @@ int clip(int count, const void* const* grads, const int64_t* sizes, const int32_
     if (short_tiles <= kShortTiles) return launch_clip_short<ORDER>(count, grads, sizes, types, outs, clip, result, st);
     if (const int rc = norm<ORDER>(count, grads, sizes, types, 0, result, tiles <= kJoinTiles ? &slots : nullptr, st)) return rc;
   }
-  if (count <= kCapSmall) return launch_clip<ORDER, kCapSmall>(count, grads, sizes, types, outs, clip, result, slots, st);
-  return launch_clip<ORDER, ClipSeg::kCapLarge>(count, grads, sizes, types, outs, clip, result, slots, st);
+  return with_constants(list_bytes(count, sizes, types) > kPlainBytes, count <= kCapSmall, [&](auto stream, auto small) {
+    constexpr int CAP = decltype(small)::value ? kCapSmall : ClipSeg::kCapLarge;
+    return launch_clip<ORDER, decltype(stream)::value, CAP>(count, grads, sizes, types, outs, clip, result, slots, st);
+  });
 }
 
-template <bool DIRECTION, int CAP>
+template <bool DIRECTION, bool STREAM, int CAP>
 int launch_momentum(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, float* const* us, float* const* outs, float m, Clip clip, double* result,
                     hipStream_t st) {
   return for_tables<MomentumSeg, CAP>(
@@ -824,7 +840,7 @@ int launch_momentum(int count, const void* const* grads, const int64_t* sizes, c
           a.tile_start[1] = 1;
           tiles = 1;
         }
-        HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, CAP>), dim3(tiles), dim3(kThreads), kWriteStreamPadLds3, st, a, clip, result, m);
+        HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, STREAM, CAP>), dim3(tiles), dim3(kThreads), STREAM ? kWriteStreamPadLds3 : 0, st, a, clip, result, m);
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
@@ -949,12 +965,15 @@ HPX_API int hpx_gd_momentum(int count, const void* const* grads, const int64_t* 
     if (const int rc = check_writes(who, count, grads, sizes, types, reinterpret_cast<const void* const*>(momenta), ds, ds)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Clip clip{result, max_norm, scale, order, result != nullptr};
-    auto launch = [&](auto direction) -> int {
-      constexpr bool D = decltype(direction)::value;
-      if (count <= kCapSmall) return launch_momentum<D, kCapSmall>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
-      return launch_momentum<D, MomentumSeg::kCapLarge>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
-    };
-    return outs ? launch(std::true_type{}) : launch(std::false_type{});
+    int64_t elements = 0;
+    for (int i = 0; i < count; i++) elements += sizes[i];
+    const bool large = list_bytes(count, sizes, types) + 4 * elements > kPlainBytes;
+    return with_constants(large, count <= kCapSmall, [&](auto streaming, auto small) {
+      constexpr bool S = decltype(streaming)::value;
+      constexpr int CAP = decltype(small)::value ? kCapSmall : MomentumSeg::kCapLarge;
+      if (outs) return launch_momentum<true, S, CAP>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
+      return launch_momentum<false, S, CAP>(count, grads, sizes, types, momenta, outs, momentum, clip, result, st);
+    });
   });
 }
 
