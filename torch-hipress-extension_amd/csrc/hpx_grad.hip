@@ -26,7 +26,7 @@ constexpr int kThreads = 256;
 // of workgroups, a cache line each.  All arrivals are zero between calls.
 constexpr int kArrivals = 3;
 constexpr int kSlots = 16;
-constexpr int kMaxGrid = 1024;  // four workgroups on each of 256 CUs
+constexpr int kMaxGrid = 512;  // two workgroups of 512 lanes on each of 256 CUs
 constexpr int kGroups = 16;
 constexpr int kGroupArrivals = kSlots + kMaxGrid;
 constexpr int kLineDoubles = 16;
@@ -172,11 +172,12 @@ struct Sum<HPX_NORM_MAX> {
   }
 };
 
-// Tiles of 16 KiB are counted from the tensor's first element, not from a boundary of memory: which elements a partial sum is
+// Tiles of 32 KiB are counted from the tensor's first element, not from a boundary of memory: which elements a partial sum is
 // made of, and so every bit of the result, then depends on types, sizes and values alone, and ranks that hold the same gradients
 // at other addresses find the same norm.
-constexpr uint32_t kNormTileBytes = 16384;
-constexpr int kNormIters = kNormTileBytes / (kThreads * 16);
+constexpr int kNormThreads = 512;
+constexpr uint32_t kNormTileBytes = 32768;
+constexpr int kNormIters = kNormTileBytes / (kNormThreads * 16);
 inline int64_t norm_tiles(int64_t n, int type) {
   const int64_t per = kNormTileBytes / (type == HPX_F32 ? 4 : 2);
   return (n + per - 1) / per;
@@ -215,7 +216,7 @@ __device__ __forceinline__ void norm_tiles_of(Sum<ORDER>& s, const void* p, int6
     Chunk<Raw> c[kNormIters];
 #pragma unroll
     for (int k = 0; k < kNormIters; k++) {
-      const Chunk<Raw>* q = reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+      const Chunk<Raw>* q = reinterpret_cast<const Chunk<Raw>*>(at + k * kNormThreads * kPer);
 #pragma unroll
       for (int i = 0; i < 4; i++) c[k].w[i] = __builtin_nontemporal_load(&q->w[i]);
     }
@@ -225,7 +226,7 @@ __device__ __forceinline__ void norm_tiles_of(Sum<ORDER>& s, const void* p, int6
   for (; t < whole; t += step, at += step * kTile) {
     Chunk<Raw> c[kNormIters];
 #pragma unroll
-    for (int k = 0; k < kNormIters; k++) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+    for (int k = 0; k < kNormIters; k++) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kNormThreads * kPer);
 #pragma unroll
     for (int k = 0; k < kNormIters; k++) norm_chunk<ORDER, TYPE>(s, c[k]);
   }
@@ -238,36 +239,81 @@ __device__ __forceinline__ void norm_tiles_of(Sum<ORDER>& s, const void* p, int6
     if (int(threadIdx.x) < rest) one = load1<TYPE>(p, n - rest + threadIdx.x);
 #pragma unroll
     for (int k = 0; k < kNormIters; k++)
-      if (k * kThreads + int(threadIdx.x) < chunks) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kThreads * kPer);
+      if (k * kNormThreads + int(threadIdx.x) < chunks) c[k] = *reinterpret_cast<const Chunk<Raw>*>(at + k * kNormThreads * kPer);
 #pragma unroll
     for (int k = 0; k < kNormIters; k++)
-      if (k * kThreads + int(threadIdx.x) < chunks) norm_chunk<ORDER, TYPE>(s, c[k]);
+      if (k * kNormThreads + int(threadIdx.x) < chunks) norm_chunk<ORDER, TYPE>(s, c[k]);
     s.add(one);
   }
 }
 
-// Over a workgroup of `waves` waves, the same order of additions whatever the timing; every lane gets the result.
+// Over a wave and over a workgroup of WAVES waves, the same order of additions whatever the timing.  By lane permutes, as
+// wave_reduce: few and short instructions, for at the end of a launch they come from memory one cache line after the other (the
+// hand-over of a norm took 2.5 us longer with four of these unrolled side by side).
 template <int ORDER>
-__device__ __forceinline__ double block_join(double v, double* lds, int waves) {
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) v = Sum<ORDER>::join(v, __shfl_xor(v, o, kWave));
+__device__ __forceinline__ double wave_join(double v) {
+  auto perm = [](double x, auto ctrl, auto rows) {
+    const uint64_t b = __double_as_longlong(x);
+    const int lo = int(uint32_t(b)), hi = int(uint32_t(b >> 32));
+    const uint32_t l = uint32_t(__builtin_amdgcn_update_dpp(lo, lo, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    const uint32_t h = uint32_t(__builtin_amdgcn_update_dpp(hi, hi, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    return __longlong_as_double(int64_t(uint64_t(h) << 32 | l));
+  };
+  using std::integral_constant;
+  using J = Sum<ORDER>;
+  v = J::join(v, perm(v, integral_constant<int, 0xB1>{}, integral_constant<int, 0xF>{}));   // quad_perm [1,0,3,2]
+  v = J::join(v, perm(v, integral_constant<int, 0x4E>{}, integral_constant<int, 0xF>{}));   // quad_perm [2,3,0,1]
+  v = J::join(v, perm(v, integral_constant<int, 0x141>{}, integral_constant<int, 0xF>{}));  // row_half_mirror
+  v = J::join(v, perm(v, integral_constant<int, 0x140>{}, integral_constant<int, 0xF>{}));  // row_mirror
+  v = J::join(v, perm(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}));  // row_bcast:15 into rows 1 and 3
+  v = J::join(v, perm(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}));  // row_bcast:31 into rows 2 and 3
+  const uint64_t b = __double_as_longlong(v);
+  const uint32_t l = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b)), kWave - 1)), h = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(b >> 32)), kWave - 1));
+  return __longlong_as_double(int64_t(uint64_t(h) << 32 | l));
+}
+template <int ORDER, int WAVES>
+__device__ __forceinline__ double block_join(double v, double* lds) {
+  v = wave_join<ORDER>(v);
   if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
   v = lds[0];
-  for (int w = 1; w < waves; w++) v = Sum<ORDER>::join(v, lds[w]);
-  __syncthreads();
+#pragma unroll
+  for (int w = 1; w < WAVES; w++) v = Sum<ORDER>::join(v, lds[w]);
   return v;
 }
 
-// The partial sums of all workgroups, in their order.
+// The partial sums of all workgroups.  One wave that takes them all, and the four waves of a workgroup that request a quarter each
+// and exchange them through LDS, add them in the same order.
+constexpr int kQuarters = 4;
 template <int ORDER>
-__device__ __forceinline__ double slots_join(const double* slots, int used, double* lds) {
-  double v = 0.0;
+__device__ __forceinline__ double slots_quarter(const double* slots, int used, int quarter) {
+  constexpr int kEach = kMaxGrid / kQuarters / kWave;
+  const int first = quarter * kEach * kWave + (threadIdx.x & (kWave - 1));
+  // (every slot is loaded, whoever may have written it: a load behind a branch of its own waits for the one before)
+  double v[kEach];
 #pragma unroll
-  for (int i = 0; i < kMaxGrid / kThreads; i++)
-    if (i * kThreads + int(threadIdx.x) < used)
-      v = Sum<ORDER>::join(v, __hip_atomic_load(&slots[i * kThreads + threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  return block_join<ORDER>(v, lds, kThreads / kWave);
+  for (int i = 0; i < kEach; i++) v[i] = __hip_atomic_load(&slots[first + i * kWave], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  double sum = first < used ? v[0] : 0.0;
+#pragma unroll
+  for (int i = 1; i < kEach; i++) sum = Sum<ORDER>::join(sum, first + i * kWave < used ? v[i] : 0.0);
+  return sum;
+}
+template <int ORDER>
+__device__ __forceinline__ double slots_join(const double* slots, int used) {
+  double v = slots_quarter<ORDER>(slots, used, 0);
+#pragma unroll
+  for (int i = 1; i < kQuarters; i++) v = Sum<ORDER>::join(v, slots_quarter<ORDER>(slots, used, i));
+  return wave_join<ORDER>(v);
+}
+template <int ORDER>
+__device__ __forceinline__ double slots_join(const double* slots, int used, double (&lds)[kQuarters][kWave]) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+  lds[wave][lane] = slots_quarter<ORDER>(slots, used, wave);
+  __syncthreads();
+  double v = lds[0][lane];
+#pragma unroll
+  for (int i = 1; i < kQuarters; i++) v = Sum<ORDER>::join(v, lds[i][lane]);
+  return wave_join<ORDER>(v);
 }
 
 template <int ORDER>
@@ -283,17 +329,17 @@ __device__ __forceinline__ void norm_result(double* result, double v, int add) {
 constexpr int64_t kKeepBytes = int64_t(192) << 20;
 
 // One pass over the list.  A workgroup sums every gridDim.x-th tile and leaves one partial sum; the last to arrive joins them in
-// their order, so the result does not depend on who that is.  Bound by memory: 604 MB at 6.3 TB/s, 102 MB in 161 tensors 20.5 us (5.0
+// their order, so the result does not depend on who that is.  Bound by memory: 604 MB at 6.3 TB/s, 102 MB in 161 tensors 19.3 us (5.3
 // TB/s, of which about 4 us are the launch and the hand-over).  The hand-over is a store, a wait and an atomic of agent scope.
 // Stores of that scope are written through, so the wait for their acknowledgement orders them before the atomic; a release fence,
 // which also writes the L2 cache back, took 45 us more with 2048 workgroups.  Atomics on one address are served about 10 ns apart,
-// hence groups: 102 MB take 28 us with 1024 arrivals at one counter.
+// hence groups: 102 MB took 28 us with 1024 arrivals at one counter, 20.5 with 16 counters and another for them.  (512 workgroups of 512
+// lanes: 19.8 then, of 256 lanes with twice the loads 21.2; 256 of 1024: 21.4.)
 // Lists of more tensors than a table holds take several launches, whose workgroups add to the slots of the one before (the first
 // `valid` of them); only the last joins.
 template <int ORDER, int CAP>
-__global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table<NormSeg, CAP> a, double* result, int valid, int last, int add) {
-  __shared__ double lds[kThreads / kWave];
-  __shared__ int am_last;
+__global__ __launch_bounds__(kNormThreads) void grad_norm_kernel(const Table<NormSeg, CAP> a, double* result, int valid, int last, int add) {
+  __shared__ double lds[kNormThreads / kWave];
   Sum<ORDER> s;
   const int tiles = a.tile_start[a.nseg], step = gridDim.x;
   const int keep = tiles - int(kKeepBytes / kNormTileBytes);
@@ -308,16 +354,17 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table<NormSeg
     }
     tile += (to - tile + step - 1) / step * step;
   }
-  double v = block_join<ORDER>(s.value(), lds, kThreads / kWave);
+  double v = block_join<ORDER, kNormThreads / kWave>(s.value(), lds);
+  if (threadIdx.x >= kWave) return;  // the first wave does the rest
   if (last && gridDim.x == 1 && valid == 0) {
     if (threadIdx.x == 0) norm_result<ORDER>(result, v, add);
     return;
   }
   double* slots = result + kSlots;
+  int am_last = 0;
   if (threadIdx.x == 0) {
     if (int(blockIdx.x) < valid) v = Sum<ORDER>::join(slots[blockIdx.x], v);
     __hip_atomic_store(&slots[blockIdx.x], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    am_last = 0;
     if (last) {
       __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const uint32_t group = blockIdx.x % kGroups, groups = gridDim.x < kGroups ? gridDim.x : kGroups;
@@ -331,9 +378,8 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(const Table<NormSeg
       }
     }
   }
-  __syncthreads();
-  if (!am_last) return;
-  v = slots_join<ORDER>(slots, int(gridDim.x) > valid ? int(gridDim.x) : valid, lds);
+  if (!__builtin_amdgcn_readfirstlane(am_last)) return;
+  v = slots_join<ORDER>(slots, int(gridDim.x) > valid ? int(gridDim.x) : valid);
   if (threadIdx.x == 0) norm_result<ORDER>(result, v, add);
 }
 
@@ -423,15 +469,16 @@ __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t 
 }
 
 // Second pass of a clipping call.  With `slots` the pass before has left its partial sums and nobody has joined them: every
-// workgroup does that for itself while its gradients are on the way, which saves the hand-over at the end of that pass and costs a
-// walk over the slots in each: 3 M elements (1500 tiles) 10.5 us against 11.9 and 12.5 against 14.2, 6 M (2900 tiles) 14.8 against
-// 16.3, 10 M (4900 tiles) 26.0 against 25.7.
-// Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 29.5 us (6.9 TB/s read and written), 110 M of a mixed
-// list 91.8 (7.2 TB/s).
-constexpr int64_t kJoinTiles = 4096;
+// workgroup does that for itself while its gradients are on the way, which saves the hand-over at the end of that pass and costs 4 KiB
+// of loads in each.  With / without, norm and clipping: 3 M fp16 elements (1500 tiles) 9.7 / 10.9 us, 10 M fp32 (4900) 22.0 / 23.5, 22 M
+// (10 700) 41.7 / 43.1, 100 M (48 800) 179.4 / 181.8, 302 M bf16 (147 500) 376.7 / 371.5.
+// Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 28.8 us (7.1 TB/s read and written), 110 M of a mixed
+// list 92 (7.2 TB/s).
+constexpr int64_t kJoinTiles = 65536;
 template <int ORDER, bool STREAM, int CAP>
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result, int slots) {
-  __shared__ double lds[kThreads / kWave];
+  static_assert(kThreads / kWave == kQuarters, "a quarter of the slots to a wave");
+  __shared__ double lds[kQuarters][kWave];
   const int tile = blockIdx.x;
   auto coefficient = [&]() -> float {
     const double s = slots ? slots_join<ORDER>(result + kSlots, slots, lds) : result[0];
@@ -467,7 +514,7 @@ __global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg
 
 // A short list in one launch of one workgroup, which keeps it in registers between the norm and the product: a wave takes 1024
 // elements of one tensor at a time, three times at most.  One CU moves some 100 GB/s, so what the second launch costs is the limit:
-// 8 thousand elements 4.5 us against 7.9 in two launches, 33 thousand 6.2 against 7.9, 60 thousand (in four rounds) 8.0 against 7.9.
+// 8 thousand elements 4.5 us against 7.9 in two launches, 33 thousand 6.2 against 7.9; 60 thousand, in four rounds, 8.0 against 7.9.
 constexpr int kShortThreads = 1024;
 constexpr int kShortTile = kWave * 16;
 constexpr int kShortRounds = 3;
@@ -531,7 +578,7 @@ __global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Ta
       for (int k = 0; k < 4; k++) { s.add(part[r].v[k].x); s.add(part[r].v[k].y); s.add(part[r].v[k].z); s.add(part[r].v[k].w); }
       s.add(part[r].one);
     }
-  const double sum = block_join<ORDER>(s.value(), lds, kShortThreads / kWave);
+  const double sum = block_join<ORDER, kShortThreads / kWave>(s.value(), lds);
   double norm = 0.0;
   const float c = clip_coefficient(clip, sum, &norm);
   if (threadIdx.x == 0) {
@@ -746,7 +793,7 @@ int launch_norm(int count, const void* const* grads, const int64_t* sizes, const
       },
       [&](const Table<NormSeg, CAP>& a, int tiles, bool last) -> int {
         const int grid = std::max(1, std::min(tiles, kMaxGrid));
-        HPX_LAUNCH("grad_norm_kernel", (grad_norm_kernel<ORDER, CAP>), dim3(grid), dim3(kThreads), st, a, result, valid, int(last && !slots), add);
+        HPX_LAUNCH("grad_norm_kernel", (grad_norm_kernel<ORDER, CAP>), dim3(grid), dim3(kNormThreads), st, a, result, valid, int(last && !slots), add);
         HPX_HIP(hipGetLastError());
         valid = std::max(valid, grid);
         return HPX_OK;
