@@ -188,6 +188,42 @@ def test_clip(pkg, which, kind, lead, out_lead):
         del now
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_lists_of_many_tiles(pkg, kind):
+    # more tiles than workgroups in every pass; beyond 96 MiB for fp32, where loads stream
+    sizes = [20_000_003, 70_001, 5, 6_000_000]
+    types = [kind, "fp32", kind, kind]
+    g, b = make(sizes, types, 40, 1)
+    before = [f64(t) for t in g]
+    want = float(sum(np.square(x).sum() for x in before))
+    norm, n = math.sqrt(want), sum(sizes)
+    result = pkg.hp_cuda_grad_result()
+    pkg.hp_cuda_grad_norm(g, sizes, result)
+    assert abs(result[0].item() - want) <= n * 2.0 ** -53 * want
+    measured = result[0].item()
+    out, ob = make(sizes, ["fp32"] * 4, 41, 3)
+    pkg.hp_cuda_grad_clip(g, sizes, out, 0.3 * norm, result)
+    assert result[0].item() == measured  # the same order of additions, whoever joins the partial sums
+    c = coefficient(norm, 0.3 * norm)
+    for x, o in zip(before, out):
+        near(o, c * x, "fp32", np.abs(c * x) * 2.0 ** -24 * (1 + 1e-6))
+    intact(ob, out)
+    for nesterov in (False, True):
+        u, ub = make(sizes, ["fp32"] * 4, 42, 2)
+        u0 = [f64(t) for t in u]
+        pkg.hp_cuda_gd_momentum(g, sizes, u, out if nesterov else None, 0.9, 0.3 * norm, result)
+        for x, v, y, z in zip(before, u0, u, out):
+            near_momentum(y, z if nesterov else None, x, v, 0.9, c)
+        intact(ub, u)
+        intact(ob, out)
+    pkg.hp_cuda_grad_clip(g, sizes, None, 2 * norm, result)
+    assert result[2].item() == 1.0 and all(np.array_equal(x, f64(t)) for x, t in zip(before, g))
+    pkg.hp_cuda_grad_clip(g, sizes, None, 0.3 * norm, result)
+    for x, t, y in zip(before, types, g):
+        near(y, c * x, t, np.abs(c * x) * 2.0 ** -23)
+    intact(b, g)
+
+
 def test_clip_leaves_what_is_short_enough(pkg):
     g, b = make([5000, 17], ["bf16", "fp32"], 5)
     bits = [t.clone() for t in b]

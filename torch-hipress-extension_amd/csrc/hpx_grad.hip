@@ -33,9 +33,10 @@ constexpr int kLineDoubles = 16;
 static_assert(kGroupArrivals + kGroups * kLineDoubles <= HPX_GRAD_RESULT, "result block too small");
 
 // ---- tables ------------------------------------------------------------------
-// An element count and its type share a word: the count needs 48 bits.
+// An element count and its type share a word.  (The limit of a count, far beyond any memory, keeps sums of them in 64 bits and the
+// tiles of a tensor in 32.)
 constexpr int kTypeShift = 56;
-constexpr int64_t kMaxSize = int64_t(1) << 48;
+constexpr int64_t kMaxSize = int64_t(1) << 40;
 __host__ __device__ inline int64_t seg_size(uint64_t nt) { return int64_t(nt & ((uint64_t(1) << kTypeShift) - 1)); }
 __host__ __device__ inline int seg_type(uint64_t nt) { return int(nt >> kTypeShift); }
 
@@ -46,7 +47,7 @@ struct NormSeg {
 };
 struct ClipSeg {
   const void* g;
-  void* out;  // g itself: in place, in g's type; else fp32
+  void* out;  // in place: g itself, in its type; else fp32
   uint64_t nt;
   static constexpr int kCapLarge = 320;
 };
@@ -475,40 +476,54 @@ __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t 
 // Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 28.8 us (7.1 TB/s read and written), 110 M of a mixed
 // list 92 (7.2 TB/s).
 constexpr int64_t kJoinTiles = 65536;
+//
+// In place there may be nothing to do, so the coefficient comes first and the tiles are shared by few workgroups: 110 M elements of a mixed
+// list that is short enough already took 77 us with a workgroup for each tile, 38 of them to start workgroups that end at once, and take
+// 41; one that is not, 117 and 107.  (1024: 40.5 and 116; 4096: 42 and 108.  Written elsewhere, 131 with a workgroup for each tile, 135 to
+// 137 so.)
+constexpr int kInPlaceGrid = 2048;
 template <int ORDER, bool STREAM, int CAP>
-__global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result, int slots) {
+__global__ __launch_bounds__(kThreads) void grad_clip_kernel(const Table<ClipSeg, CAP> a, const Clip clip, double* result, int slots, int in_place) {
   static_assert(kThreads / kWave == kQuarters, "a quarter of the slots to a wave");
   __shared__ double lds[kQuarters][kWave];
-  const int tile = blockIdx.x;
   auto coefficient = [&]() -> float {
     const double s = slots ? slots_join<ORDER>(result + kSlots, slots, lds) : result[0];
     double norm = 0.0;
     const float c = clip_coefficient(clip, s, &norm);
-    if (clip.tell && tile == 0 && threadIdx.x == 0) {
+    if (clip.tell && blockIdx.x == 0 && threadIdx.x == 0) {
       if (slots) result[0] = s;
       result[1] = norm;
       result[2] = double(c);
     }
     return c;
   };
-  const int k = find_segment<CAP>(a.tile_start, a.nseg, tile);
+  if (in_place) {
+    const float c = coefficient();
+    if (c == 1.f) return;
+    auto known = [c]() { return c; };
+    for (int tile = blockIdx.x; tile < a.tile_start[a.nseg]; tile += gridDim.x) {
+      const int k = find_segment<CAP>(a.tile_start, a.nseg, tile);
+      const ClipSeg sg = a.seg[k];
+      const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
+      switch (seg_type(sg.nt)) {
+        case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, known); break;
+        case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16, STREAM>(sg, n, t, known); break;
+        default: clip_tile<HPX_F16, HPX_F16, STREAM>(sg, n, t, known); break;
+      }
+    }
+    return;
+  }
+  if (a.nseg == 0) {  // norm and coefficient are told all the same
+    coefficient();
+    return;
+  }
+  const int tile = blockIdx.x, k = find_segment<CAP>(a.tile_start, a.nseg, tile);
   const ClipSeg sg = a.seg[k];
   const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
-  if (sg.out == sg.g) {  // in place, or nothing at all
-    const float c = coefficient();
-    if (c == 1.f || n == 0) return;
-    auto known = [c]() { return c; };
-    switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, known); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_BF16, STREAM>(sg, n, t, known); break;
-      default: clip_tile<HPX_F16, HPX_F16, STREAM>(sg, n, t, known); break;
-    }
-  } else {
-    switch (seg_type(sg.nt)) {
-      case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, coefficient); break;
-      case HPX_BF16: clip_tile<HPX_BF16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
-      default: clip_tile<HPX_F16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
-    }
+  switch (seg_type(sg.nt)) {
+    case HPX_F32: clip_tile<HPX_F32, HPX_F32, STREAM>(sg, n, t, coefficient); break;
+    case HPX_BF16: clip_tile<HPX_BF16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
+    default: clip_tile<HPX_F16, HPX_F32, STREAM>(sg, n, t, coefficient); break;
   }
 }
 
@@ -550,7 +565,7 @@ __device__ __forceinline__ void short_store(const ShortPart& p, void* out, int64
 }
 
 template <int ORDER>
-__global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Table<ClipSeg, kShortTiles> a, const Clip clip, double* result) {
+__global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Table<ClipSeg, kShortTiles> a, const Clip clip, double* result, int in_place) {
   __shared__ double lds[kShortThreads / kWave];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), tiles = a.tile_start[a.nseg];
   ShortPart part[kShortRounds];
@@ -586,6 +601,7 @@ __global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Ta
     result[1] = norm;
     result[2] = double(c);
   }
+  if (in_place && c == 1.f) return;
 #pragma unroll
   for (int r = 0; r < kShortRounds; r++) {
     const int tile = r * (kShortThreads / kWave) + wave;
@@ -593,9 +609,7 @@ __global__ __launch_bounds__(kShortThreads) void grad_clip_short_kernel(const Ta
       const int k = seg[r];
       const ClipSeg sg = a.seg[k];
       const int64_t n = seg_size(sg.nt), first = int64_t(tile - a.tile_start[k]) * kShortTile;
-      const int out = sg.out == sg.g ? seg_type(sg.nt) : HPX_F32;
-      if (sg.out == sg.g && c == 1.f) continue;
-      switch (out) {
+      switch (in_place ? seg_type(sg.nt) : HPX_F32) {
         case HPX_F32: short_store<HPX_F32>(part[r], sg.out, n, first, c); break;
         case HPX_BF16: short_store<HPX_BF16>(part[r], sg.out, n, first, c); break;
         default: short_store<HPX_F16>(part[r], sg.out, n, first, c); break;
@@ -669,10 +683,10 @@ __global__ __launch_bounds__(kThreads) void gd_momentum_kernel(const Table<Momen
     result[1] = norm;
     result[2] = double(c);
   }
+  if (a.nseg == 0) return;
   const int k = find_segment<CAP>(a.tile_start, a.nseg, tile);
   const MomentumSeg sg = a.seg[k];
   const int64_t n = seg_size(sg.nt), t = tile - a.tile_start[k];
-  if (n == 0) return;
   switch (seg_type(sg.nt)) {
     case HPX_F32: momentum_tile<HPX_F32, DIRECTION, STREAM>(sg, n, t, m, c); break;
     case HPX_BF16: momentum_tile<HPX_BF16, DIRECTION, STREAM>(sg, n, t, m, c); break;
@@ -764,11 +778,7 @@ int for_tables(int count, Fill fill, Launch launch) {
     while (i < count && a.nseg < CAP) {
       const int64_t tiles = fill(i, a.seg[a.nseg]);
       if (tiles == 0) { i++; continue; }
-      if (int64_t(a.tile_start[a.nseg]) + tiles > INT32_MAX - kMaxGrid) {
-        if (a.nseg) break;
-        set_error("tensor %d is too large for one launch", i);
-        return HPX_ERR_ARG;
-      }
+      if (int64_t(a.tile_start[a.nseg]) + tiles > INT32_MAX - kMaxGrid) break;  // never the first: see kMaxSize
       a.tile_start[a.nseg + 1] = a.tile_start[a.nseg] + int32_t(tiles);
       a.nseg++;
       i++;
@@ -809,25 +819,26 @@ int norm(int count, const void* const* grads, const int64_t* sizes, const int32_
 
 ClipSeg clip_seg(const void* g, void* out, int64_t size, int type) { return ClipSeg{g, out, uint64_t(size) | uint64_t(type) << kTypeShift}; }
 
+// Outputs of a clipping call: null where it works in place.
+struct Outs {
+  float* const* p;
+  void* at(const void* const* grads, int i) const { return p ? static_cast<void*>(p[i]) : const_cast<void*>(grads[i]); }
+  int item(int type) const { return p ? 4 : item_size(type); }
+};
+
 template <int ORDER, bool STREAM, int CAP>
-int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, Clip clip, double* result, int slots, hipStream_t st) {
+int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, Clip clip, double* result, int slots, hipStream_t st) {
   return for_tables<ClipSeg, CAP>(
       count,
       [&](int i, ClipSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
-        sg = clip_seg(grads[i], outs[i], sizes[i], type);
-        return write_tiles<kClipIters>(outs[i], sizes[i], outs[i] == grads[i] ? item_size(type) : 4);
+        sg = clip_seg(grads[i], outs.at(grads, i), sizes[i], type);
+        return write_tiles<kClipIters>(sg.out, sizes[i], outs.item(type));
       },
-      [&](Table<ClipSeg, CAP>& a, int tiles, bool) -> int {
-        if (tiles == 0) {  // norm and coefficient are told all the same
-          if (!clip.tell) return HPX_OK;
-          a.seg[0] = ClipSeg{nullptr, nullptr, 0};
-          a.nseg = 1;
-          a.tile_start[1] = 1;
-          tiles = 1;
-        }
-        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<ORDER, STREAM, CAP>), dim3(tiles), dim3(kThreads), st, a, clip, result, slots);
+      [&](const Table<ClipSeg, CAP>& a, int tiles, bool) -> int {
+        const int grid = std::max(1, outs.p ? tiles : std::min(tiles, kInPlaceGrid));
+        HPX_LAUNCH("grad_clip_kernel", (grad_clip_kernel<ORDER, STREAM, CAP>), dim3(grid), dim3(kThreads), st, a, clip, result, slots, int(!outs.p));
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
@@ -836,28 +847,28 @@ int launch_clip(int count, const void* const* grads, const int64_t* sizes, const
 
 // Lists of up to kShortTiles tiles of 1024 elements: one launch of one workgroup.
 template <int ORDER>
-int launch_clip_short(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, const Clip& clip, double* result, hipStream_t st) {
+int launch_clip_short(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, const Clip& clip, double* result, hipStream_t st) {
   return for_tables<ClipSeg, kShortTiles>(
       count,
       [&](int i, ClipSeg& sg) -> int64_t {
-        sg = clip_seg(grads[i], outs[i], sizes[i], types ? types[i] : HPX_F32);
+        sg = clip_seg(grads[i], outs.at(grads, i), sizes[i], types ? types[i] : HPX_F32);
         return (sizes[i] + kShortTile - 1) / kShortTile;
       },
       [&](const Table<ClipSeg, kShortTiles>& a, int, bool) -> int {
-        HPX_LAUNCH("grad_clip_short_kernel", (grad_clip_short_kernel<ORDER>), dim3(1), dim3(kShortThreads), st, a, clip, result);
+        HPX_LAUNCH("grad_clip_short_kernel", (grad_clip_short_kernel<ORDER>), dim3(1), dim3(kShortThreads), st, a, clip, result, int(!outs.p));
         HPX_HIP(hipGetLastError());
         return HPX_OK;
       });
 }
 
 template <int ORDER>
-int clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, void* const* outs, bool measured, const Clip& clip, double* result, hipStream_t st) {
+int clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, bool measured, const Clip& clip, double* result, hipStream_t st) {
   int slots = 0;
   if (!measured) {
     int64_t short_tiles = 0, tiles = 0;
     for (int i = 0; i < count; i++) {
       short_tiles += (sizes[i] + kShortTile - 1) / kShortTile;
-      tiles += sizes[i] ? (sizes[i] + 2 * kThreads * 4 * kClipIters - 2) / (kThreads * 4 * kClipIters) : 0;  // at most
+      tiles += sizes[i] / (kThreads * 4 * kClipIters) + 1;
     }
     if (short_tiles <= kShortTiles) return launch_clip_short<ORDER>(count, grads, sizes, types, outs, clip, result, st);
     if (const int rc = norm<ORDER>(count, grads, sizes, types, 0, result, tiles <= kJoinTiles ? &slots : nullptr, st)) return rc;
@@ -879,15 +890,8 @@ int launch_momentum(int count, const void* const* grads, const int64_t* sizes, c
         sg = MomentumSeg{grads[i], us[i], outs ? outs[i] : nullptr, uint64_t(sizes[i]) | uint64_t(type) << kTypeShift};
         return write_tiles<kMomentumIters<DIRECTION>>(us[i], sizes[i], 4);
       },
-      [&](Table<MomentumSeg, CAP>& a, int tiles, bool) -> int {
-        if (tiles == 0) {
-          if (!clip.tell) return HPX_OK;
-          a.seg[0] = MomentumSeg{nullptr, nullptr, nullptr, 0};
-          a.nseg = 1;
-          a.tile_start[1] = 1;
-          tiles = 1;
-        }
-        HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, STREAM, CAP>), dim3(tiles), dim3(kThreads), STREAM ? kWriteStreamPadLds3 : 0, st, a, clip, result, m);
+      [&](const Table<MomentumSeg, CAP>& a, int tiles, bool) -> int {
+        HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, STREAM, CAP>), dim3(std::max(1, tiles)), dim3(kThreads), STREAM ? kWriteStreamPadLds3 : 0, st, a, clip, result, m);
         HPX_HIP(hipGetLastError());
         clip.tell = 0;
         return HPX_OK;
@@ -978,17 +982,17 @@ HPX_API int hpx_grad_clip(int count, const void* const* grads, const int64_t* si
     if (const int rc = check_clip(who, order, max_norm, scale)) return rc;
     if (const int rc = check_result(who, result)) return rc;
     if (const int rc = check_list(who, count, grads, sizes, types)) return rc;
-    std::vector<void*> to(static_cast<size_t>(count));
-    for (int i = 0; i < count; i++) {
-      to[size_t(i)] = outs ? outs[i] : const_cast<void*>(grads[i]);
-      HPX_ARG(sizes[i] == 0 || (to[size_t(i)] && (!outs || aligned(outs[i], 4))), "%s: output %d is null or does not start at a multiple of its element size", who, i);
-      HPX_ARG(sizes[i] == 0 || !outs || !types || types[i] == HPX_F32 || outs[i] != grads[i], "%s: output %d is fp32 and cannot take the place of a gradient of another type", who, i);
+    for (int i = 0; outs && i < count; i++) {
+      if (sizes[i] == 0) continue;
+      HPX_ARG(outs[i] && aligned(outs[i], 4), "%s: output %d is null or does not start at a multiple of its element size", who, i);
+      HPX_ARG(!types || types[i] == HPX_F32 || outs[i] != grads[i], "%s: output %d is fp32 and cannot take the place of a gradient of another type", who, i);
     }
-    if (const int rc = check_writes(who, count, grads, sizes, types, to.data(), nullptr, to.data())) return rc;
+    const void* const* to = outs ? reinterpret_cast<const void* const*>(outs) : grads;
+    if (const int rc = check_writes(who, count, grads, sizes, types, to, nullptr, to)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Clip how{result, max_norm, scale, order, 1};
-    return order == 2 ? clip<2>(count, grads, sizes, types, to.data(), is_measured != 0, how, result, st)
-                      : clip<HPX_NORM_MAX>(count, grads, sizes, types, to.data(), is_measured != 0, how, result, st);
+    return order == 2 ? clip<2>(count, grads, sizes, types, Outs{outs}, is_measured != 0, how, result, st)
+                      : clip<HPX_NORM_MAX>(count, grads, sizes, types, Outs{outs}, is_measured != 0, how, result, st);
   });
 }
 
