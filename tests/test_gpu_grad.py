@@ -105,6 +105,34 @@ def test_norm_of_several_lists(pkg):
     assert result[0].item() == max(float(np.abs(f64(t)).max()) for g in lists for t in g)
 
 
+def test_norm_of_two_tables_the_second_with_more_tiles(pkg):
+    # 448 small tensors fill the first table; the second has more workgroups than the first
+    sizes = [1 + i % 7 for i in range(448)] + [9_000_001, 8_000_003]
+    g, _ = make(sizes, types_of("fp32", sizes), 50, 1)
+    g[449] = g[449].bfloat16()
+    want = float(sum(np.square(f64(t)).sum() for t in g))
+    for _ in range(2):
+        result = pkg.hp_cuda_grad_result()
+        result[16:528] = float("nan")  # slots that no call has written yet may hold anything
+        pkg.hp_cuda_grad_norm(g, sizes, result)
+        assert abs(result[0].item() - want) <= sum(sizes) * 2.0 ** -53 * want
+        pkg.hp_cuda_grad_norm(g, sizes, result, 0)
+        assert result[0].item() == max(float(np.abs(f64(t)).max()) for t in g)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "mixed"])
+@pytest.mark.parametrize("which", ["tiny", "edges", "ragged", "many", "large"])
+def test_norm_has_the_same_bits_at_other_addresses(pkg, which, kind):
+    sizes = SIZES[which]
+    seen = set()
+    for lead in (0, 1, 3, 64):
+        g, _ = make(sizes, types_of(kind, sizes), 51, lead)
+        result = pkg.hp_cuda_grad_result()
+        pkg.hp_cuda_grad_norm(g, sizes, result)
+        seen.add((result[0].item(), result[1].item()))
+    assert len(seen) == 1
+
+
 def test_norm_of_nothing(pkg):
     result = pkg.hp_cuda_grad_result().fill_(0)
     for g, sizes in (([], []), ([torch.zeros(0, device="cuda")], [0])):
@@ -493,6 +521,41 @@ def test_two_graphs_of_one_stream(pkg):
             assert torch.equal(s["result"][:3], result[:3])
             assert all(torch.equal(x, y) for x, y in zip(s["out"], out)) and all(torch.equal(x, y) for x, y in zip(s["u"], u))
         assert math.isfinite(float(torch.randn(1 << 20, device="cuda").sum()))
+
+
+def test_calls_from_several_threads(pkg):
+    # each thread with a stream, a result block and tensors of its own
+    import threading
+    sizes, types = [200_001, 33, 5000], ["bf16", "fp32", "fp16"]
+    jobs = []
+    for k in range(4):
+        g, _ = make(sizes, types, 60 + k)
+        norm = math.sqrt(squares(g))
+        jobs.append((g, norm, [torch.zeros(n, device="cuda") for n in sizes], [torch.zeros(n, device="cuda") for n in sizes],
+                     pkg.hp_cuda_grad_result(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(g, norm, out, u, result, stream):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    pkg.hp_cuda_grad_clip(g, sizes, out, 0.5 * norm, result)
+                    pkg.hp_cuda_grad_norm(g, sizes, result)
+                    pkg.hp_cuda_gd_momentum(g, sizes, u, None, 0.0, 0.5 * norm, result)
+                stream.synchronize()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads: t.start()
+    for t in threads: t.join()
+    assert not failed
+    for g, norm, out, u, result, _ in jobs:
+        c = coefficient(norm, 0.5 * norm)
+        for x, o, v in zip(g, out, u):
+            near(o, c * f64(x), "fp32", np.abs(c * f64(x)) * 2.0 ** -24 * (1 + 1e-6))
+            assert torch.equal(o, v)
 
 
 def test_more_elements_than_32_bits_count(pkg):
