@@ -23,7 +23,8 @@
  *   - The library owns a small grow-only device workspace per (device, stream).
  *     Entry points may be called from several host threads; calls that share a
  *     stream are serialised while they enqueue.
- *   - Sizes are int32 element/byte counts exactly as in the reference.
+ *   - Sizes are int32 element/byte counts exactly as in the reference (those of the
+ *     gradient operators, which have no counterpart there, are int64).
  *   - Tuning options: see hpx_set_option.
  */
 #ifndef HPX_H_
