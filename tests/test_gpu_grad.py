@@ -261,6 +261,32 @@ def test_clip_leaves_what_is_short_enough(pkg):
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(bits, b))
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "mixed"])
+@pytest.mark.parametrize("which", ["tiny", "ragged", "many", "large"])
+def test_clip_by_the_largest_magnitude(pkg, which, kind):
+    sizes = SIZES[which]
+    types = types_of(kind, sizes)
+    g, b = make(sizes, types, 70, 1)
+    before = [f64(t) for t in g]
+    most = max(float(np.abs(x).max()) for x in before if x.size)
+    result = pkg.hp_cuda_grad_result()
+    out, ob = make(sizes, ["fp32"] * len(sizes), 71, 2)
+    c = coefficient(most, 0.5 * most)
+    pkg.hp_cuda_grad_clip(g, sizes, out, 0.5 * most, result, order=0)
+    assert result[:2].tolist() == [most, most] and abs(result[2].item() - c) <= c * 2.0 ** -24 * (1 + 1e-6)
+    u, _ = make(sizes, ["fp32"] * len(sizes), 72)
+    u0 = [f64(t) for t in u]
+    pkg.hp_cuda_gd_momentum(g, sizes, u, None, 0.9, 0.5 * most, result, 0)
+    for x, v, o, y in zip(before, u0, out, u):
+        near(o, c * x, "fp32", np.abs(c * x) * 2.0 ** -24 * (1 + 1e-6))
+        near_momentum(y, None, x, v, 0.9, c)
+    pkg.hp_cuda_grad_clip(g, sizes, None, 0.5 * most, result, order=0)
+    for x, t, y in zip(before, types, g):
+        near(y, c * x, t, np.abs(c * x) * 2.0 ** -23)
+    intact(b, g)
+    intact(ob, out)
+
+
 @pytest.mark.parametrize("order", [2, 0])
 def test_clip_by_a_norm_over_ranks(pkg, order):
     # what an all-reduce leaves in result[0]
