@@ -92,6 +92,32 @@ def test_norm(pkg, which, kind, lead):
     assert result[3:16].tolist() == [0.0] * 13  # the count of arrivals is back at zero
 
 
+@pytest.mark.parametrize("full", [8, 48, 256, 320, 448])
+@pytest.mark.parametrize("n", [3, 2000])
+def test_empty_tensors_behind_a_full_table(pkg, full, n):
+    sizes = [n] * full + [0, 0]
+    g, b = make(sizes, types_of("mixed", sizes), 80, 1)
+    before = [f64(t) for t in g]
+    want = squares(g)
+    norm = math.sqrt(want)
+    c = coefficient(norm, 0.5 * norm)
+    result = pkg.hp_cuda_grad_result()
+    pkg.hp_cuda_grad_norm(g, sizes, result)
+    assert abs(result[0].item() - want) <= sum(sizes) * 2.0 ** -53 * want
+    out, _ = make(sizes, ["fp32"] * len(sizes), 81)
+    u, _ = make(sizes, ["fp32"] * len(sizes), 82)
+    u0 = [f64(t) for t in u]
+    pkg.hp_cuda_grad_clip(g, sizes, out, 0.5 * norm, result)
+    pkg.hp_cuda_gd_momentum(g, sizes, u, None, 0.9, 0.5 * norm, result)
+    for x, o, v, y in zip(before, out, u0, u):
+        near(o, c * x, "fp32", np.abs(c * x) * 2.0 ** -24 * (1 + 1e-6))
+        near_momentum(y, None, x, v, 0.9, c)
+    pkg.hp_cuda_grad_clip(g, sizes, None, 0.5 * norm, result)
+    assert abs(result[0].item() - want) <= sum(sizes) * 2.0 ** -53 * want
+    assert abs(result[1].item() / norm - 1) <= 1e-9 and abs(result[2].item() - c) <= c * 2.0 ** -24 * (1 + 1e-6)
+    intact(b, g)
+
+
 def test_norm_of_several_lists(pkg):
     sizes = [70_001, 33, 4096]
     lists = [make(sizes, [t] * 3, seed)[0] for seed, t in enumerate(("fp32", "bf16", "fp16"))]

@@ -788,13 +788,14 @@ int for_tables(int count, Fill fill, Launch launch) {
   do {
     a.nseg = 0;
     a.tile_start[0] = 0;
-    while (i < count && a.nseg < CAP) {
-      const int64_t tiles = fill(i, a.seg[a.nseg]);
-      if (tiles == 0) { i++; continue; }
-      if (int64_t(a.tile_start[a.nseg]) + tiles > INT32_MAX - kMaxGrid) break;  // never the first: see kMaxSize
+    for (; i < count; i++) {  // to the next item that has tiles, also when the table is full: a launch knows whether it is the last
+      Seg seg;
+      const int64_t tiles = fill(i, seg);
+      if (tiles == 0) continue;
+      if (a.nseg == CAP || int64_t(a.tile_start[a.nseg]) + tiles > INT32_MAX - kMaxGrid) break;  // the latter never for the first: see kMaxSize
+      a.seg[a.nseg] = seg;
       a.tile_start[a.nseg + 1] = a.tile_start[a.nseg] + int32_t(tiles);
       a.nseg++;
-      i++;
     }
     const int rc = launch(a, a.tile_start[a.nseg], i == count);
     if (rc != HPX_OK) return rc;
