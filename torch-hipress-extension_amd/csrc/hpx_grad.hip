@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "hpx_common.h"
+#include "hpx_tables.h"
 
 namespace {
 using namespace hpx;
@@ -34,7 +35,7 @@ static_assert(kGroupArrivals + kGroups * kLineDoubles <= HPX_GRAD_RESULT, "resul
 
 // ---- tables ------------------------------------------------------------------
 // An element count and its type share a word.  (The limit of a count, far beyond any memory, keeps sums of them in 64 bits and the
-// tiles of a tensor in 32.)
+// tiles of a tensor in the norm, which takes it as a whole, in 32.)
 constexpr int kTypeShift = 56;
 constexpr int64_t kMaxSize = int64_t(1) << 40;
 __host__ __device__ inline int64_t seg_size(uint64_t nt) { return int64_t(nt & ((uint64_t(1) << kTypeShift) - 1)); }
@@ -67,12 +68,6 @@ struct MaskSeg {
 };
 constexpr int kCapSmall = 8;
 
-template <typename Seg, int CAP>
-struct Table {
-  int32_t nseg;
-  int32_t tile_start[CAP + 1];
-  Seg seg[CAP];
-};
 static_assert(sizeof(Table<NormSeg, NormSeg::kCapLarge>) <= 9600 && sizeof(Table<ClipSeg, ClipSeg::kCapLarge>) <= 9600 &&
                   sizeof(Table<MomentumSeg, MomentumSeg::kCapLarge>) <= 9600 && sizeof(Table<MaskSeg, MaskSeg::kCapLarge>) <= 9600,
               "kernel-argument budget");
@@ -779,37 +774,17 @@ int check_clip(const char* who, int order, double max_norm, double scale) {
   return HPX_OK;
 }
 
-// Fills tables from items [0, count) and hands each to `launch(table, tiles, last)`.  fill(i, seg) returns the number of
-// tiles of item i, 0 to leave it out.  At least one launch is made, of an empty table if need be.
-template <typename Seg, int CAP, typename Fill, typename Launch>
-int for_tables(int count, Fill fill, Launch launch) {
-  Table<Seg, CAP> a;
-  int i = 0;
-  do {
-    a.nseg = 0;
-    a.tile_start[0] = 0;
-    for (; i < count; i++) {  // to the next item that has tiles, also when the table is full: a launch knows whether it is the last
-      Seg seg;
-      const int64_t tiles = fill(i, seg);
-      if (tiles == 0) continue;
-      if (a.nseg == CAP || int64_t(a.tile_start[a.nseg]) + tiles > INT32_MAX - kMaxGrid) break;  // the latter never for the first: see kMaxSize
-      a.seg[a.nseg] = seg;
-      a.tile_start[a.nseg + 1] = a.tile_start[a.nseg] + int32_t(tiles);
-      a.nseg++;
-    }
-    const int rc = launch(a, a.tile_start[a.nseg], i == count);
-    if (rc != HPX_OK) return rc;
-  } while (i < count);
-  return HPX_OK;
-}
+// `elements` of `item` bytes behind p.
+const void* behind(const void* p, int64_t elements, int item) { return static_cast<const uint8_t*>(p) + elements * item; }
+void* behind(void* p, int64_t elements, int item) { return static_cast<uint8_t*>(p) + elements * item; }
 
 // slots: not null where the caller joins the partial sums itself; gets their number.
 template <int ORDER, int CAP>
 int launch_norm(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, int add, double* result, int* slots, hipStream_t st) {
   int valid = 0;
   const int rc = for_tables<NormSeg, CAP>(
-      count,
-      [&](int i, NormSeg& sg) -> int64_t {
+      count, INT32_MAX - kMaxGrid,  // a fixed grid walks over the tiles: only their number has to stay in 32 bits
+      [&](int i, int64_t*, NormSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
         sg = NormSeg{grads[i], uint64_t(sizes[i]) | uint64_t(type) << kTypeShift};
@@ -843,12 +818,13 @@ struct Outs {
 template <int ORDER, bool STREAM, int CAP>
 int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, Clip clip, double* result, int slots, hipStream_t st) {
   return for_tables<ClipSeg, CAP>(
-      count,
-      [&](int i, ClipSeg& sg) -> int64_t {
+      count, most_tiles(kThreads),
+      [&](int i, int64_t* at, ClipSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
-        sg = clip_seg(grads[i], outs.at(grads, i), sizes[i], type);
-        return write_tiles<kClipIters>(sg.out, sizes[i], outs.item(type));
+        const int64_t from = *at, n = next_part(sizes[i], at);
+        sg = clip_seg(behind(grads[i], from, item_size(type)), behind(outs.at(grads, i), from, outs.item(type)), n, type);
+        return write_tiles<kClipIters>(sg.out, n, outs.item(type));
       },
       [&](const Table<ClipSeg, CAP>& a, int tiles, bool) -> int {
         const int grid = std::max(1, outs.p ? tiles : std::min(tiles, kInPlaceGrid));
@@ -863,8 +839,8 @@ int launch_clip(int count, const void* const* grads, const int64_t* sizes, const
 template <int ORDER>
 int launch_clip_short(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, const Clip& clip, double* result, hipStream_t st) {
   return for_tables<ClipSeg, kShortTiles>(
-      count,
-      [&](int i, ClipSeg& sg) -> int64_t {
+      count, kShortTiles,
+      [&](int i, int64_t*, ClipSeg& sg) -> int64_t {
         sg = clip_seg(grads[i], outs.at(grads, i), sizes[i], types ? types[i] : HPX_F32);
         return (sizes[i] + kShortTile - 1) / kShortTile;
       },
@@ -897,12 +873,13 @@ template <bool DIRECTION, bool STREAM, int CAP>
 int launch_momentum(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, float* const* us, float* const* outs, float m, Clip clip, double* result,
                     hipStream_t st) {
   return for_tables<MomentumSeg, CAP>(
-      count,
-      [&](int i, MomentumSeg& sg) -> int64_t {
+      count, most_tiles(kThreads),
+      [&](int i, int64_t* at, MomentumSeg& sg) -> int64_t {
         if (sizes[i] == 0) return 0;
         const int type = types ? types[i] : HPX_F32;
-        sg = MomentumSeg{grads[i], us[i], outs ? outs[i] : nullptr, uint64_t(sizes[i]) | uint64_t(type) << kTypeShift};
-        return write_tiles<kMomentumIters<DIRECTION>>(us[i], sizes[i], 4);
+        const int64_t from = *at, n = next_part(sizes[i], at);
+        sg = MomentumSeg{behind(grads[i], from, item_size(type)), us[i] + from, outs ? outs[i] + from : nullptr, uint64_t(n) | uint64_t(type) << kTypeShift};
+        return write_tiles<kMomentumIters<DIRECTION>>(sg.u, n, 4);
       },
       [&](const Table<MomentumSeg, CAP>& a, int tiles, bool) -> int {
         HPX_LAUNCH_LDS("gd_momentum_kernel", hpx::g_prof_on, (gd_momentum_kernel<DIRECTION, STREAM, CAP>), dim3(std::max(1, tiles)), dim3(kThreads), STREAM ? kWriteStreamPadLds3 : 0, st, a, clip, result, m);
@@ -916,8 +893,8 @@ template <int CAP>
 int launch_mask(int count, const uint8_t* const* ins, const int32_t* in_sizes, float* const* us, const int32_t* sizes, int32_t* counts, hipStream_t st) {
   int first = 0;
   return for_tables<MaskSeg, CAP>(
-      count,
-      [&](int i, MaskSeg& sg) -> int64_t {
+      count, most_tiles(kThreads),
+      [&](int i, int64_t*, MaskSeg& sg) -> int64_t {
         sg = MaskSeg{ins[i], us[i], in_sizes[i], sizes[i]};
         return std::max(1, (mask_room(in_sizes[i]) + kMaskTile - 1) / kMaskTile);
       },
