@@ -417,7 +417,9 @@ int hpx_gd_momentum(int count, const void* const* grads, const int64_t* sizes,
  * device; in_sizes[t] is the message's room.  Indices outside [0, sizes[t]) are
  * passed over; a message whose header is not 4 + 8k or exceeds in_sizes[t] masks
  * nothing.  counts: NULL, or `count` device words that get the number of entries
- * of each message, -1 for such a header. */
+ * of each message, -1 for such a header.  Several messages may name one momentum, or
+ * momenta that overlap.  -3 if a message overlaps a momentum, or the counts overlap
+ * either. */
 int hpx_gd_mask(int count, const uint8_t* const* ins, const int32_t* in_sizes,
                 float* const* momenta, const int32_t* sizes, int32_t* counts,
                 hpx_stream_t stream);

@@ -108,6 +108,21 @@ def test_messages(capi, change, text):
     assert text in capi.last_error()
 
 
+def test_messages_and_counts_apart_from_what_is_written(capi):
+    # a message of 20 bytes against momenta of 8 elements, whole and by its last or first word
+    for ins, us in (((A,), (A,)), ((A,), (A + 16,)), ((A + 28,), (A,)), ((2 * A, 4 * A + 28), (8 * A, 4 * A))):
+        n = len(ins)
+        assert _mask(capi, ins=ins, in_sizes=(20,) * n, us=us, sizes=(8,) * n) == -3
+        assert f"message {n - 1} overlaps a momentum" in capi.last_error()
+    # momenta that overlap each other hide none of the first
+    assert _mask(capi, ins=(A + 40, 4 * A), in_sizes=(20, 20), us=(A, A + 16), sizes=(64, 2)) == -3 and "message 0" in capi.last_error()
+    assert _mask(capi, us=(2 * A,), counts=2 * A + 28) == -3 and "the counts overlap a momentum" in capi.last_error()
+    assert _mask(capi, ins=(A, A + 64), in_sizes=(20, 20), us=(2 * A, 3 * A), sizes=(8, 8), counts=A - 4) == -3
+    assert "the counts overlap message 0" in capi.last_error()
+    assert _mask(capi, ins=(A, A + 64), in_sizes=(20, 20), us=(2 * A, 3 * A), sizes=(8, 8), counts=A + 80) == -3
+    assert "the counts overlap message 1" in capi.last_error()
+
+
 def test_python_functions_are_there(pkg):
     for name in ("hp_cuda_grad_result", "hp_cuda_grad_norm", "hp_cuda_grad_clip", "hp_cuda_gd_momentum", "hp_cuda_gd_mask"):
         assert callable(getattr(pkg, name)) and name in pkg.__all__

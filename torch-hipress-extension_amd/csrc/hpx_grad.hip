@@ -743,14 +743,25 @@ int with_constants(bool a, bool b, F f) {
 struct Span {
   uintptr_t b, e;
 };
-// Whether the spans, in any order, overlap anywhere; sorts them.
+Span span(const void* p, int64_t bytes) { return {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + uintptr_t(bytes)}; }
+// Whether the spans, in any order, overlap anywhere; sorts them and joins those that do.
 bool overlap(std::vector<Span>& v) {
   bool sorted = true;
   for (size_t i = 1; i < v.size() && sorted; i++) sorted = v[i - 1].b <= v[i].b;
   if (!sorted) std::sort(v.begin(), v.end(), [](const Span& x, const Span& y) { return x.b < y.b; });
-  for (size_t i = 1; i < v.size(); i++)
-    if (v[i].b < v[i - 1].e) return true;
-  return false;
+  size_t n = 0;
+  for (const Span& x : v) {
+    if (n > 0 && x.b < v[n - 1].e) v[n - 1].e = std::max(v[n - 1].e, x.e);
+    else v[n++] = x;
+  }
+  const bool found = n < v.size();
+  v.resize(n);
+  return found;
+}
+// Whether x overlaps one of the spans that overlap() has been through.
+bool meets(const std::vector<Span>& v, const Span& x) {
+  auto it = std::upper_bound(v.begin(), v.end(), x.b, [](uintptr_t at, const Span& s) { return at < s.e; });  // the first that ends behind x's begin
+  return it != v.end() && it->b < x.e;
 }
 
 int check_list(const char* who, int count, const void* const* grads, const int64_t* sizes, const int32_t* types) {
@@ -915,23 +926,17 @@ int check_writes(const char* who, int count, const void* const* grads, const int
   w.reserve(size_t(count) * (b ? 2 : 1));
   for (int i = 0; i < count; i++) {
     if (sizes[i] == 0) continue;
-    const int item = a[i] == grads[i] ? item_size(types ? types[i] : HPX_F32) : 4;
-    const uintptr_t p = reinterpret_cast<uintptr_t>(a[i]);
-    w.push_back({p, p + uintptr_t(sizes[i]) * item});
+    w.push_back(span(a[i], sizes[i] * (a[i] == grads[i] ? item_size(types ? types[i] : HPX_F32) : 4)));
   }
   for (int i = 0; b && i < count; i++) {
     if (sizes[i] == 0) continue;
-    const uintptr_t p = reinterpret_cast<uintptr_t>(b[i]);
-    w.push_back({p, p + uintptr_t(sizes[i]) * 4});
+    w.push_back(span(b[i], sizes[i] * 4));
   }
   HPX_ARG(!overlap(w), "%s: two of the tensors that are written overlap", who);
   for (int i = 0; i < count; i++) {
     if (sizes[i] == 0) continue;
-    const uintptr_t p = reinterpret_cast<uintptr_t>(grads[i]), e = p + uintptr_t(sizes[i]) * item_size(types ? types[i] : HPX_F32);
     if (in_place && in_place[i] == grads[i]) continue;
-    // the first written span that ends behind p
-    auto it = std::upper_bound(w.begin(), w.end(), p, [](uintptr_t x, const Span& s) { return x < s.e; });
-    HPX_ARG(it == w.end() || it->b >= e, "%s: gradient %d overlaps a tensor that is written", who, i);
+    HPX_ARG(!meets(w, span(grads[i], sizes[i] * item_size(types ? types[i] : HPX_F32))), "%s: gradient %d overlaps a tensor that is written", who, i);
   }
   return HPX_OK;
 }
@@ -1031,6 +1036,20 @@ HPX_API int hpx_gd_mask(int count, const uint8_t* const* ins, const int32_t* in_
       HPX_ARG(in_sizes[i] >= 0 && sizes[i] >= 0, "%s: message %d has a negative size", who, i);
       HPX_ARG(in_sizes[i] < 4 || (ins[i] && aligned(ins[i], 4)), "%s: message %d is null or does not start at a multiple of 4 bytes", who, i);
       HPX_ARG(sizes[i] == 0 || (momenta[i] && aligned(momenta[i], 4)), "%s: momentum %d is null or does not start at a multiple of 4 bytes", who, i);
+    }
+    // Zeros are all that is stored to momenta, so several messages may name one; what is read must not be among it, nor the counts.
+    std::vector<Span> w;
+    w.reserve(size_t(count));
+    for (int i = 0; i < count; i++)
+      if (sizes[i] > 0) w.push_back(span(momenta[i], int64_t(sizes[i]) * 4));
+    overlap(w);
+    const Span told = span(counts, counts ? int64_t(count) * 4 : 0);
+    HPX_ARG(!counts || !meets(w, told), "%s: the counts overlap a momentum", who);
+    for (int i = 0; i < count; i++) {
+      if (in_sizes[i] < 4) continue;
+      const Span in = span(ins[i], in_sizes[i]);
+      HPX_ARG(!meets(w, in), "%s: message %d overlaps a momentum", who, i);
+      HPX_ARG(!counts || in.e <= told.b || told.e <= in.b, "%s: the counts overlap message %d", who, i);
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (count <= kCapSmall) return launch_mask<kCapSmall>(count, ins, in_sizes, momenta, sizes, counts, st);
