@@ -362,7 +362,8 @@ int hpx_dgc_decode(int count, const uint8_t* const* ins, const int32_t* in_sizes
  *              Tensors start at any multiple of their element size.
  *   result     HPX_GRAD_RESULT doubles of device memory that the caller owns and
  *              has zeroed once: [0] S, [1] norm, [2] coefficient, the rest room
- *              for the calls (zeroing it again is never needed).  A call in flight
+ *              for the calls (zeroing it again is never needed).  -3 if a tensor
+ *              of the call overlaps it.  A call in flight
  *              has its block to itself; calls with blocks of their own, also
  *              graphs captured on one stream, share nothing.
  *   order      2: S = sum of squares over all tensors, N = sqrt(S);

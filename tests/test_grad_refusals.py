@@ -94,6 +94,18 @@ def test_overlapping_tensors(capi):
     assert _momentum(capi, us=(A + 28,), outs=(4 * A,)) == -3
 
 
+@pytest.mark.parametrize("at", [0, 8, 24, 2063 * 8])
+def test_tensors_apart_from_the_result_block(capi, at):
+    R = 16 * A
+    for call, kinds in ((_norm, ("ptrs",)), (_clip, ("ptrs", "outs")), (_momentum, ("ptrs", "us", "outs"))):
+        for kind in kinds:
+            name = {"ptrs": "gradient", "us": "momentum", "outs": "output"}[kind]
+            assert call(capi, result=R, **{kind: (R + at,)}) == -3 and f"{name} 0 overlaps the result block" in capi.last_error()
+            # from below: eight elements whose last is the block's first
+            assert call(capi, result=R, **{kind: (R - 28,)}) == -3 and f"{name} 0 overlaps the result block" in capi.last_error()
+    assert _clip(capi, ptrs=(A, R + at), sizes=(8, 2), types=(0, 1), result=R) == -3 and "gradient 1 overlaps" in capi.last_error()
+
+
 @pytest.mark.parametrize("change, text", [
     (dict(in_sizes=(-1,)), "negative size"),
     (dict(sizes=(-1,)), "negative size"),

@@ -778,6 +778,18 @@ int check_result(const char* who, const double* result) {
   HPX_ARG(result && aligned(result, 8), "%s: the result block is null or does not start at a multiple of 8 bytes", who);
   return HPX_OK;
 }
+// A tensor that shares memory with the block would be read while sums are stored there, or overwrite its counters of arrivals, which
+// later calls rely on.  (null: an operator without a list of that kind, or without a block)
+int check_apart(const char* who, const char* what, int count, const void* const* p, const int64_t* sizes, const int32_t* types, const double* result) {
+  if (!p || !result) return HPX_OK;
+  const Span block = span(result, HPX_GRAD_RESULT * int64_t(sizeof(double)));
+  for (int i = 0; i < count; i++) {
+    if (sizes[i] == 0) continue;
+    const Span s = span(p[i], sizes[i] * item_size(types ? types[i] : HPX_F32));
+    HPX_ARG(s.e <= block.b || block.e <= s.b, "%s: %s %d overlaps the result block", who, what, i);
+  }
+  return HPX_OK;
+}
 int check_clip(const char* who, int order, double max_norm, double scale) {
   HPX_ARG(order == 2 || order == HPX_NORM_MAX, "%s: order %d is neither 2 nor HPX_NORM_MAX", who, order);
   HPX_ARG(max_norm >= 0.0, "%s: max_norm %g is negative or not a number", who, max_norm);
@@ -963,6 +975,7 @@ HPX_API int hpx_grad_norm(int count, const void* const* grads, const int64_t* si
     if (const int rc = check_clip(who, order, 0.0, 1.0)) return rc;
     if (const int rc = check_result(who, result)) return rc;
     if (const int rc = check_list(who, count, grads, sizes, types)) return rc;
+    if (const int rc = check_apart(who, "gradient", count, grads, sizes, types, result)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return order == 2 ? norm<2>(count, grads, sizes, types, is_add_to != 0, result, nullptr, st)
                       : norm<HPX_NORM_MAX>(count, grads, sizes, types, is_add_to != 0, result, nullptr, st);
@@ -985,6 +998,8 @@ HPX_API int hpx_grad_clip(int count, const void* const* grads, const int64_t* si
     }
     const void* const* to = outs ? reinterpret_cast<const void* const*>(outs) : grads;
     if (const int rc = check_writes(who, count, grads, sizes, types, to, nullptr, to)) return rc;
+    if (const int rc = check_apart(who, "gradient", count, grads, sizes, types, result)) return rc;
+    if (const int rc = check_apart(who, "output", count, outs ? to : nullptr, sizes, nullptr, result)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Clip how{result, max_norm, scale, order, 1};
     return order == 2 ? clip<2>(count, grads, sizes, types, Outs{outs}, is_measured != 0, how, result, st)
@@ -1008,8 +1023,11 @@ HPX_API int hpx_gd_momentum(int count, const void* const* grads, const int64_t* 
       HPX_ARG(!outs || (outs[i] && aligned(outs[i], 4)), "%s: output %d is null or does not start at a multiple of its element size", who, i);
       HPX_ARG(!outs || !types || types[i] == HPX_F32 || outs[i] != grads[i], "%s: output %d is fp32 and cannot take the place of a gradient of another type", who, i);
     }
-    const void* const* ds = reinterpret_cast<const void* const*>(outs);
-    if (const int rc = check_writes(who, count, grads, sizes, types, reinterpret_cast<const void* const*>(momenta), ds, ds)) return rc;
+    const void* const *us = reinterpret_cast<const void* const*>(momenta), *const *ds = reinterpret_cast<const void* const*>(outs);
+    if (const int rc = check_writes(who, count, grads, sizes, types, us, ds, ds)) return rc;
+    if (const int rc = check_apart(who, "gradient", count, grads, sizes, types, result)) return rc;
+    if (const int rc = check_apart(who, "momentum", count, us, sizes, nullptr, result)) return rc;
+    if (const int rc = check_apart(who, "output", count, ds, sizes, nullptr, result)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Clip clip{result, max_norm, scale, order, result != nullptr};
     int64_t elements = 0;
