@@ -22,3 +22,18 @@ def test_several_messages_for_one_momentum(pkg):
         want[i] = 0
     want[n - 100 + np.array(index[3])] = 0
     assert np.array_equal(f64(whole), want) and counts.tolist() == [len(i) for i in index]
+
+
+def test_orders_that_an_int_does_not_hold(pkg):
+    x, r = torch.ones(64, device="cuda"), pkg.hp_cuda_grad_result()
+    for order in ((1 << 32) + 2, 1 << 32, (1 << 64) + 2):
+        with pytest.raises(ValueError, match="order"):
+            pkg.hp_cuda_grad_norm([x], [64], r, order)
+        with pytest.raises(ValueError, match="order"):
+            pkg.hp_cuda_grad_clip([x], [64], None, 1.0, r, order=order)
+        with pytest.raises(ValueError, match="order"):
+            pkg.hp_cuda_gd_momentum([x], [64], [torch.ones(64, device="cuda")], None, 0.9, 1.0, r, order)
+    assert bool((x == 1).all()) and bool((r == 0).all())
+    # numbers of other kinds than int are taken as before
+    pkg.hp_cuda_grad_norm([x], [np.int64(64)], r, np.int32(2))
+    assert r[0].item() == 64.0

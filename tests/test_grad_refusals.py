@@ -135,6 +135,25 @@ def test_messages_and_counts_apart_from_what_is_written(capi):
     assert "the counts overlap message 1" in capi.last_error()
 
 
+def test_sizes_that_their_type_does_not_hold(pkg):
+    # none of them is its lower bits
+    for size in ((1 << 64) + 8, 1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="sizes"):
+            pkg.hp_cuda_grad_norm([A], [size], 2 * A, stream=0)
+        with pytest.raises(ValueError, match="sizes"):
+            pkg.hp_cuda_grad_clip([A], [size], None, 1.0, 2 * A, stream=0)
+        with pytest.raises(ValueError, match="sizes"):
+            pkg.hp_cuda_gd_momentum([A], [size], [4 * A], None, 0.9, 1.0, 2 * A, stream=0)
+    for size in ((1 << 32) + 8, 1 << 31, -(1 << 31) - 1, (1 << 64) + 8):
+        with pytest.raises(ValueError, match="sizes"):
+            pkg.hp_cuda_gd_mask([A], [20], [2 * A], [size], stream=0)
+        with pytest.raises(ValueError, match="in sizes"):
+            pkg.hp_cuda_gd_mask([A], [size], [2 * A], [8], stream=0)
+    for code in ((1 << 32) + 1, (1 << 64) + 1):
+        with pytest.raises(ValueError, match="types"):
+            pkg.hp_cuda_grad_norm([A], [8], 2 * A, types=[code], stream=0)
+
+
 def test_python_functions_are_there(pkg):
     for name in ("hp_cuda_grad_result", "hp_cuda_grad_norm", "hp_cuda_grad_clip", "hp_cuda_gd_momentum", "hp_cuda_gd_mask"):
         assert callable(getattr(pkg, name)) and name in pkg.__all__

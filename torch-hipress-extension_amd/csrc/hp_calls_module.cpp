@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include <limits>
 #include <vector>
 
 #include "hpx.h"
@@ -284,6 +285,30 @@ PyObject* powersgd_decode(PyObject* const* a) {  // Ps, Qs, Ms, residuals, grads
   return released([&] { return hpx_powersgd_decode(int(n), ro(pp), ro(qp), mp.data(), rp.data(), gp.data(), numel.data(), d.n.data(), d.m.data(), d.r.data(), st); });
 }
 
+// int(v), refused where T does not hold it: a size or a code must not turn into another by its lower bits.
+template <typename T>
+T whole(PyObject* v, const char* what) {
+  PyObject* i = PyNumber_Long(v);
+  if (!i) throw PyError{};
+  int over = 0;
+  const long long x = PyLong_AsLongLongAndOverflow(i, &over);
+  Py_DECREF(i);
+  if (x == -1 && !over && PyErr_Occurred()) throw PyError{};
+  if (over || x < static_cast<long long>(std::numeric_limits<T>::min()) || x > static_cast<long long>(std::numeric_limits<T>::max())) {
+    PyErr_Format(PyExc_ValueError, "%s: a number out of range", what);
+    throw PyError{};
+  }
+  return static_cast<T>(x);
+}
+template <typename T>
+std::vector<T> wholes(PyObject* o, Py_ssize_t count, const char* what) {
+  Seq s(o);
+  need(s.n, count, what);
+  std::vector<T> v(static_cast<size_t>(s.n));
+  for (Py_ssize_t i = 0; i < s.n; i++) v[size_t(i)] = whole<T>(s.items[i], what);
+  return v;
+}
+
 // The gradients of a list, which may be of several types: addresses, sizes and type codes.  Tensors bring their type, and are
 // checked against `sizes` and the current device; an address is of the type that `types` gives (None: fp32), which a tensor
 // has to agree with.
@@ -323,17 +348,17 @@ void fits(const at::Tensor& t, int64_t size, int at, const char* what) {
 
 Grads gradients(PyObject* list, PyObject* sizes, PyObject* types) {
   Seq s(list);
-  const int device = c10::hip::current_device();  // asked once: 30 ns a tensor otherwise
   Grads g;
-  g.size = ints<int64_t>(sizes, s.n, "sizes");
+  g.size = wholes<int64_t>(sizes, s.n, "sizes");
   g.p.resize(size_t(s.n));
   g.type.assign(size_t(s.n), HPX_F32);
   if (types != Py_None) {
     Seq t(types);
     need(t.n, s.n, "types");
     for (Py_ssize_t i = 0; i < s.n; i++)
-      g.type[size_t(i)] = THPDtype_Check(t.items[i]) ? type_code(reinterpret_cast<THPDtype*>(t.items[i])->scalar_type, "gradients") : static_cast<int32_t>(as_int(t.items[i]));
+      g.type[size_t(i)] = THPDtype_Check(t.items[i]) ? type_code(reinterpret_cast<THPDtype*>(t.items[i])->scalar_type, "gradients") : whole<int32_t>(t.items[i], "types");
   }
+  const int device = c10::hip::current_device();  // asked once: 30 ns a tensor otherwise
   for (Py_ssize_t i = 0; i < s.n; i++) {
     if (THPVariable_Check(s.items[i])) {
       const at::Tensor& t = THPVariable_Unpack(s.items[i]);
@@ -408,7 +433,7 @@ int as_flag(PyObject* o) {
 PyObject* grad_norm(PyObject* const* a) {  // grads, sizes, result, order, is_add_to, types, stream
   const Grads g = gradients(a[0], a[1], a[5]);
   double* result = result_block(a[2]);
-  const int order = int(as_int(a[3])), add = as_flag(a[4]);
+  const int order = whole<int>(a[3], "order"), add = as_flag(a[4]);
   hipStream_t st = stream_of(a[6]);
   return released_or_raised([&] { return hpx_grad_norm(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), order, add, result, st); });
 }
@@ -420,7 +445,7 @@ PyObject* grad_clip(PyObject* const* a) {  // grads, sizes, outs, max_norm, resu
   float* const* outs = a[2] != Py_None ? out.data() : nullptr;
   const double max_norm = as_float(a[3]), scale = as_float(a[7]);
   double* result = result_block(a[4]);
-  const int measured = as_flag(a[5]), order = int(as_int(a[6]));
+  const int measured = as_flag(a[5]), order = whole<int>(a[6], "order");
   hipStream_t st = stream_of(a[9]);
   return released_or_raised([&] { return hpx_grad_clip(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), outs, measured, order, max_norm, scale, result, st); });
 }
@@ -433,7 +458,7 @@ PyObject* gd_momentum(PyObject* const* a) {  // grads, sizes, momenta, outs, mom
   float* const* outs = a[3] != Py_None ? out.data() : nullptr;
   const double m = as_float(a[4]), max_norm = as_float(a[5]), scale = as_float(a[8]);
   double* result = a[6] != Py_None ? result_block(a[6]) : nullptr;
-  const int order = int(as_int(a[7]));
+  const int order = whole<int>(a[7], "order");
   hipStream_t st = stream_of(a[10]);
   return released_or_raised(
       [&] { return hpx_gd_momentum(int(g.p.size()), g.p.data(), g.size.data(), g.type.data(), u.data(), outs, float(m), order, max_norm, scale, result, st); });
@@ -442,7 +467,7 @@ PyObject* gd_momentum(PyObject* const* a) {  // grads, sizes, momenta, outs, mom
 PyObject* gd_mask(PyObject* const* a) {  // ins, in_sizes, momenta, sizes, counts, stream
   Seq s(a[0]);
   const size_t n = size_t(s.n);
-  const auto in_size = ints<int32_t>(a[1], s.n, "in sizes"), size = ints<int32_t>(a[3], s.n, "sizes");
+  const auto in_size = wholes<int32_t>(a[1], s.n, "in sizes"), size = wholes<int32_t>(a[3], s.n, "sizes");
   const auto in = companions<uint8_t>(a[0], in_size, n, at::kByte, "a message");
   const auto u = companions<float>(a[2], size, n, at::kFloat, "a momentum");
   int32_t* counts = nullptr;
