@@ -154,6 +154,15 @@ def test_sizes_that_their_type_does_not_hold(pkg):
             pkg.hp_cuda_grad_norm([A], [8], 2 * A, types=[code], stream=0)
 
 
+def test_result_block_is_on_the_device_that_is_named(pkg, monkeypatch):
+    import torch
+    asked = []
+    monkeypatch.setattr(torch, "zeros", lambda *shape, dtype, device: asked.append((shape, dtype, device)))
+    for device in (None, 0, 1, "cuda:1"):
+        pkg.hp_cuda_grad_result(device)
+    assert asked == [((2064,), torch.float64, d) for d in ("cuda", 0, 1, "cuda:1")]
+
+
 def test_python_functions_are_there(pkg):
     for name in ("hp_cuda_grad_result", "hp_cuda_grad_norm", "hp_cuda_grad_clip", "hp_cuda_gd_momentum", "hp_cuda_gd_mask"):
         assert callable(getattr(pkg, name)) and name in pkg.__all__

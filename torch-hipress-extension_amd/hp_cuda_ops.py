@@ -96,8 +96,9 @@ def hp_cuda_powersgd_decode(Ps, Qs, Ms, residuals, grads, stream=None):
 
 def hp_cuda_grad_result(device=None):
     """A result block for the three functions below: float64, zeroed.  [0] is the sum of squares (or the largest magnitude), what
-    ranks all-reduce; [1] the norm; [2] the coefficient; the rest is room for the calls.  One block per chain of calls."""
-    return torch.zeros(_capi.GRAD_RESULT, dtype=torch.float64, device=device or "cuda")
+    ranks all-reduce; [1] the norm; [2] the coefficient; the rest is room for the calls.  One block per chain of calls.  device: None is
+    the current one."""
+    return torch.zeros(_capi.GRAD_RESULT, dtype=torch.float64, device="cuda" if device is None else device)
 
 
 def hp_cuda_grad_norm(grads, sizes, result, order=2, is_add_to=0, types=None, stream=None):
