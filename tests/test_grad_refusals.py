@@ -163,6 +163,20 @@ def test_result_block_is_on_the_device_that_is_named(pkg, monkeypatch):
     assert asked == [((2064,), torch.float64, d) for d in ("cuda", 0, 1, "cuda:1")]
 
 
+def test_streams_of_another_device(pkg, monkeypatch):
+    import torch
+
+    class Stream:
+        device_index, cuda_stream = 1, 0
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    for call in (lambda s: pkg.hp_cuda_grad_norm([], [], A, stream=s), lambda s: pkg.hp_cuda_grad_clip([], [], None, 1.0, A, stream=s),
+                 lambda s: pkg.hp_cuda_gd_momentum([], [], [], None, 0.9, 1.0, None, stream=s), lambda s: pkg.hp_cuda_gd_mask([], [], [], [], stream=s)):
+        with pytest.raises(RuntimeError, match="one of device 1, the current device is 0"):
+            call(Stream())
+
+
 def test_python_functions_are_there(pkg):
     for name in ("hp_cuda_grad_result", "hp_cuda_grad_norm", "hp_cuda_grad_clip", "hp_cuda_gd_momentum", "hp_cuda_gd_mask"):
         assert callable(getattr(pkg, name)) and name in pkg.__all__

@@ -94,6 +94,13 @@ def hp_cuda_powersgd_decode(Ps, Qs, Ms, residuals, grads, stream=None):
 # ---- gradients before and after the codecs (no counterpart in the reference, whose caller does this in torch) -----------
 # Refused arguments raise: these have no driver of the reference's to be like.
 
+def _stream_here(stream):
+    """As _stream, for calls whose tensors have to lie on the current device: a kernel on another device's stream could not read them."""
+    if isinstance(stream, torch.cuda.Stream) and stream.device_index != torch.cuda.current_device():
+        raise RuntimeError(f"the stream is one of device {stream.device_index}, the current device is {torch.cuda.current_device()}")
+    return _stream(stream)
+
+
 def hp_cuda_grad_result(device=None):
     """A result block for the three functions below: float64, zeroed.  [0] is the sum of squares (or the largest magnitude), what
     ranks all-reduce; [1] the norm; [2] the coefficient; the rest is room for the calls.  One block per chain of calls.  device: None is
@@ -105,24 +112,24 @@ def hp_cuda_grad_norm(grads, sizes, result, order=2, is_add_to=0, types=None, st
     """result[0] = the sum of squares over all gradients (order 2) or their largest magnitude (order 0), in fp64; result[1] the
     norm.  is_add_to: the list joins what result[0] holds.  float32, bfloat16 and float16 may stand in one list; `types` (torch
     dtypes) says what raw addresses point to.  Does not wait."""
-    _calls().grad_norm(grads, sizes, result, order, is_add_to, types, _stream(stream))
+    _calls().grad_norm(grads, sizes, result, order, is_add_to, types, _stream_here(stream))
 
 
 def hp_cuda_grad_clip(grads, sizes, outs, max_norm, result, is_measured=0, order=2, scale=1.0, types=None, stream=None):
     """out = c * grad, c = scale * min(1, max_norm / (|scale| * norm + 1e-6)), 0 where the norm is not finite.  outs None: in place, in
     the gradient's type; else float32 tensors, which the codecs encode.  The norm of the list is taken first, or with is_measured
     from result[0].  result[1] = |scale| * norm, result[2] = c.  Does not wait."""
-    _calls().grad_clip(grads, sizes, outs, max_norm, result, is_measured, order, scale, types, _stream(stream))
+    _calls().grad_clip(grads, sizes, outs, max_norm, result, is_measured, order, scale, types, _stream_here(stream))
 
 
 def hp_cuda_gd_momentum(grads, sizes, momenta, outs, momentum, max_norm, result, order=2, scale=1.0, types=None, stream=None):
     """Momentum correction before hp_cuda_gd: momenta = momentum * momenta + c * grad with c from result[0] as above (result None:
     c = scale), and where outs are given Nesterov's direction outs = momentum * momenta + c * grad.  What hp_cuda_gd takes as
     the gradient is momenta, or outs.  Does not wait."""
-    _calls().gd_momentum(grads, sizes, momenta, outs, momentum, max_norm, result, order, scale, types, _stream(stream))
+    _calls().gd_momentum(grads, sizes, momenta, outs, momentum, max_norm, result, order, scale, types, _stream_here(stream))
 
 
 def hp_cuda_gd_mask(in_uint8_ts, in_uint8_t_sizes, momenta, momenta_sizes, counts=None, stream=None):
     """Momentum factor masking behind hp_cuda_gd: zeroes the momenta at the indices that the messages carry.  counts: an int32 tensor
     for the number of entries of each message, -1 where its header is none.  Does not wait."""
-    _calls().gd_mask(in_uint8_ts, in_uint8_t_sizes, momenta, momenta_sizes, counts, _stream(stream))
+    _calls().gd_mask(in_uint8_ts, in_uint8_t_sizes, momenta, momenta_sizes, counts, _stream_here(stream))
