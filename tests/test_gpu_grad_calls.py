@@ -1,9 +1,12 @@
-"""Calls of the gradient operators that their documentation allows, beside those of test_gpu_grad.py."""
+"""Calls of the gradient operators that their documentation allows, beside those of test_gpu_grad.py; the tolerances are
+those derived there."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_grad import f64, make, message
+from test_gpu_grad import SIZES, coefficient, f64, intact, make, message, near, near_momentum, squares, types_of
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +40,79 @@ def test_orders_that_an_int_does_not_hold(pkg):
     # numbers of other kinds than int are taken as before
     pkg.hp_cuda_grad_norm([x], [np.int64(64)], r, np.int32(2))
     assert r[0].item() == 64.0
+
+
+def told(result, s, norm, c, scale=1.0):
+    assert abs(result[0].item() - s) <= 1e-9 * s
+    assert abs(result[1].item() / (abs(scale) * norm) - 1) <= 1e-9
+    assert abs(result[2].item() - c) <= abs(c) * 2.0 ** -24 * (1 + 1e-6)
+
+
+@pytest.mark.parametrize("measured", [0, 1])
+@pytest.mark.parametrize("lead", [0, 1, 3])
+@pytest.mark.parametrize("which", list(SIZES))
+def test_fp32_outputs_in_the_place_of_the_gradients(pkg, which, lead, measured):
+    sizes = SIZES[which]
+    for share, scale in ((0.3, 1.0), (0.3, -0.5), (2.0, 0.125)):  # of the norm
+        g, b = make(sizes, ["fp32"] * len(sizes), 90, lead)
+        before = [f64(t) for t in g]
+        total = squares(g)
+        norm = math.sqrt(total)
+        result = pkg.hp_cuda_grad_result()
+        if measured:
+            result[0] = total
+        pkg.hp_cuda_grad_clip(g, sizes, g, share * abs(scale) * norm, result, measured, scale=scale)
+        c = coefficient(norm, share * abs(scale) * norm, scale)
+        assert c != 0 and c != 1
+        told(result, total, norm, c, scale)
+        for x, y in zip(before, g):
+            near(y, c * x, "fp32", np.abs(c * x) * 2.0 ** -24 * (1 + 1e-6), which)
+        intact(b, g)
+
+
+@pytest.mark.parametrize("which", ["tiny", "ragged", "many", "large"])
+def test_some_outputs_in_the_place_of_their_gradients(pkg, which):
+    sizes = SIZES[which]
+    types = types_of("mixed", sizes)
+    g, b = make(sizes, types, 91, 1)
+    other, ob = make(sizes, ["fp32"] * len(sizes), 92, 2)
+    own = [t == "fp32" and i % 2 == 0 for i, t in enumerate(types)]
+    out = [x if mine else o for x, o, mine in zip(g, other, own)]
+    before = [f64(t) for t in g]
+    norm = math.sqrt(squares(g))
+    result = pkg.hp_cuda_grad_result()
+    pkg.hp_cuda_grad_clip(g, sizes, out, 0.3 * norm, result)
+    c = coefficient(norm, 0.3 * norm)
+    for x, o, y, mine in zip(before, out, g, own):
+        near(o, c * x, "fp32", np.abs(c * x) * 2.0 ** -24 * (1 + 1e-6), which)
+        assert mine or np.array_equal(f64(y), x)
+    # Nesterov's direction likewise
+    u, ub = make(sizes, ["fp32"] * len(sizes), 93, 3)
+    u0, before = [f64(t) for t in u], [f64(t) for t in g]
+    pkg.hp_cuda_gd_momentum(g, sizes, u, out, 0.9, 1.0, None, scale=-0.25)
+    for x, v, y, d in zip(before, u0, u, out):
+        near_momentum(y, d, x, v, 0.9, -0.25)
+    for bs, ts in ((b, g), (ob, other), (ub, u)):
+        intact(bs, ts)
+
+
+@pytest.mark.parametrize("measured", [0, 1])
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16", "mixed"])
+@pytest.mark.parametrize("which", list(SIZES))
+def test_unscaling_in_place(pkg, which, kind, measured):
+    sizes = SIZES[which]
+    types = types_of(kind, sizes)
+    for share, scale, lead in ((2.0, 2.0 ** -10, 0), (0.3, -0.375, 1), (2.0, 3.0, 5)):
+        g, b = make(sizes, types, 94, lead)
+        before = [f64(t) for t in g]
+        total = squares(g)
+        norm = math.sqrt(total)
+        result = pkg.hp_cuda_grad_result()
+        if measured:
+            result[0] = total
+        pkg.hp_cuda_grad_clip(g, sizes, None, share * abs(scale) * norm, result, measured, scale=scale)
+        c = coefficient(norm, share * abs(scale) * norm, scale)
+        told(result, total, norm, c, scale)
+        for x, t, y in zip(before, types, g):
+            near(y, c * x, t, np.abs(c * x) * 2.0 ** -23, (which, kind))
+        intact(b, g)
