@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from gpu_util import stream_ptr
 from test_gpu_grad import SIZES, coefficient, f64, intact, make, message, near, near_momentum, squares, types_of
 
 pytestmark = pytest.mark.gpu
@@ -116,3 +117,28 @@ def test_unscaling_in_place(pkg, which, kind, measured):
         for x, t, y in zip(before, types, g):
             near(y, c * x, t, np.abs(c * x) * 2.0 ** -23, (which, kind))
         intact(b, g)
+
+
+def test_masks_by_messages_of_the_sparsifier_without_residual(pkg, capi, oracle_cpu):
+    # hpx_dgc_encode clears what it sends in the tensor that it is given: here a copy of the momentum
+    sizes, seeds = [1000, 65_536, 100_003, 33], [3, 1 << 22, 12_345 << 20, 5]
+    rates, shares = [0.05, 0.5, 0.01, 1.0], [0.01, 0.5, 0.001, 0.1]
+    u, b = make(sizes, ["fp32"] * len(sizes), 95, 1)
+    before = [t.clone() for t in u]
+    sent = [t.clone() for t in u]
+    rooms = [4 + 8 * math.ceil(n * s) for n, s in zip(sizes, shares)]
+    msgs = [torch.full((r,), 0xEE, dtype=torch.uint8, device="cuda") for r in rooms]
+    counts = torch.zeros(len(sizes), dtype=torch.int32, device="cuda")
+    rc = capi.load().hpx_dgc_encode(len(sizes), capi.ptr_array([t.data_ptr() for t in sent]), capi.i32_array(sizes),
+                                    capi.ptr_array([m.data_ptr() for m in msgs]), capi.f64_array(rates), capi.f64_array(shares),
+                                    capi.u64_array(seeds), stream_ptr())
+    assert rc == 0, capi.last_error()
+    pkg.hp_cuda_gd_mask(msgs, rooms, u, sizes, counts)
+    for i, n in enumerate(sizes):
+        ref, _ = oracle_cpu.dgc_encode(before[i].cpu().numpy(), rates[i], shares[i], seeds[i])
+        k = (ref.size - 4) // 8
+        assert counts[i].item() == k and (k > 0) == (i > 0)  # the first tensor's samples hold its largest value: nothing lies beyond them
+        want = f64(before[i])
+        want[ref[4:4 + 4 * k].view(np.int32)] = 0
+        assert np.array_equal(f64(u[i]), want)
+    intact(b, u)
