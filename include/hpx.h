@@ -368,8 +368,13 @@ int hpx_dgc_decode(int count, const uint8_t* const* ins, const int32_t* in_sizes
  *              graphs captured on one stream, share nothing.
  *   order      2: S = sum of squares over all tensors, N = sqrt(S);
  *              HPX_NORM_MAX: S = N = the largest magnitude.  S is computed and
- *              kept in fp64; its bits depend on the types, sizes and values of the
- *              list alone, not on addresses or timing.  A NaN anywhere gives NaN.
+ *              kept in fp64; its bits depend on the call and on the types, sizes and
+ *              values of the list alone, not on addresses or timing.  The two calls that
+ *              take it, hpx_grad_norm and an hpx_grad_clip that is not told it, add
+ *              short lists in different orders (those of up to 48 tiles, a tensor having
+ *              one for each 1024 elements or part of them), and their sums of squares may
+ *              differ there by roundings of fp64: ranks that have to find the same
+ *              coefficient make the same calls.  A NaN anywhere gives NaN.
  *   coefficient c = scale * min(1, max_norm / (|scale| N + 1e-6)), rounded to
  *              fp32 once; N that is infinite or a NaN gives c = 0.  max_norm may be
  *              infinity (no clipping).  c = 0 takes nothing of a gradient, whatever it
@@ -394,7 +399,7 @@ int hpx_grad_norm(int count, const void* const* grads, const int64_t* sizes,
 /* out = c * g for every element.  outs == NULL: in place, in the gradient's own
  * type; with c = 1 nothing is touched.  Otherwise outs[t] is fp32 - what the
  * codecs encode - and may be grads[t] where that is fp32.  is_measured == 0: the
- * norm of this list is taken first, as by hpx_grad_norm; otherwise result[0] holds
+ * norm of this list is taken first and S left in result[0]; otherwise result[0] holds
  * S already.  result[1] = |scale| N, result[2] = c.  -3 if two tensors that are
  * written overlap, or one that is written and another gradient. */
 int hpx_grad_clip(int count, const void* const* grads, const int64_t* sizes,

@@ -142,3 +142,31 @@ def test_masks_by_messages_of_the_sparsifier_without_residual(pkg, capi, oracle_
         want[ref[4:4 + 4 * k].view(np.int32)] = 0
         assert np.array_equal(f64(u[i]), want)
     intact(b, u)
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "fp16", "mixed"])
+@pytest.mark.parametrize("sizes", [[1], [2048], [1, 3, 7, 0, 9, 1023, 1024, 1025], [33, 16_385, 5000], [49_152], [49_153], [1000] * 48, [1000] * 49])
+def test_sum_of_a_clip_that_measures(pkg, sizes, kind):
+    # the lists of up to 48 tiles and the shortest beyond: the same bits at every address, in place and not, and but for the order
+    # of additions hp_cuda_grad_norm's
+    types, n = types_of(kind, sizes), sum(sizes)
+    seen, most = set(), set()
+    for lead in (0, 1, 3, 64):
+        g, _ = make(sizes, types, 96, lead)
+        out, _ = make(sizes, ["fp32"] * len(sizes), 97, lead + 1)
+        norm, result = pkg.hp_cuda_grad_result(), pkg.hp_cuda_grad_result()
+        pkg.hp_cuda_grad_norm(g, sizes, norm)
+        pkg.hp_cuda_grad_clip(g, sizes, out, 0.01, result)
+        seen.add((norm[0].item(), *result[:3].tolist()))
+        pkg.hp_cuda_grad_clip(g, sizes, out, 0.01, result, order=0)
+        pkg.hp_cuda_grad_norm(g, sizes, norm, 0)
+        most.add((norm[0].item(), *result[:2].tolist()))
+        pkg.hp_cuda_grad_clip(g, sizes, None, 0.01, result)
+        seen.add((seen.copy().pop()[0], *result[:3].tolist()))
+    assert len(seen) == 1 and len(most) == 1
+    (of_norm, of_clip, length, c), = seen
+    assert abs(of_clip - of_norm) <= 2 * n * 2.0 ** -53 * of_norm
+    # the root, the divisor, the quotient and the rounding to fp32
+    assert abs(c - coefficient(math.sqrt(of_clip), 0.01)) <= abs(c) * 2.0 ** -24 * (1 + 1e-6)
+    (a, b, length), = most
+    assert a == b == length

@@ -118,7 +118,8 @@ def hp_cuda_grad_norm(grads, sizes, result, order=2, is_add_to=0, types=None, st
 def hp_cuda_grad_clip(grads, sizes, outs, max_norm, result, is_measured=0, order=2, scale=1.0, types=None, stream=None):
     """out = c * grad, c = scale * min(1, max_norm / (|scale| * norm + 1e-6)), 0 where the norm is not finite.  outs None: in place, in
     the gradient's type; else float32 tensors, which the codecs encode.  The norm of the list is taken first, or with is_measured
-    from result[0].  result[1] = |scale| * norm, result[2] = c.  Does not wait."""
+    from result[0].  result[1] = |scale| * norm, result[2] = c.  Does not wait.  A short list's sum of squares may differ from
+    hp_cuda_grad_norm's by roundings of fp64 (include/hpx.h): ranks that have to find the same c make the same calls."""
     _calls().grad_clip(grads, sizes, outs, max_norm, result, is_measured, order, scale, types, _stream_here(stream))
 
 
