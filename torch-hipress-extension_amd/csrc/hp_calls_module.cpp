@@ -288,11 +288,16 @@ PyObject* powersgd_decode(PyObject* const* a) {  // Ps, Qs, Ms, residuals, grads
 // int(v), refused where T does not hold it: a size or a code must not turn into another by its lower bits.
 template <typename T>
 T whole(PyObject* v, const char* what) {
-  PyObject* i = PyNumber_Long(v);
-  if (!i) throw PyError{};
   int over = 0;
-  const long long x = PyLong_AsLongLongAndOverflow(i, &over);
-  Py_DECREF(i);
+  long long x;
+  if (PyLong_CheckExact(v)) {
+    x = PyLong_AsLongLongAndOverflow(v, &over);
+  } else {
+    PyObject* i = PyNumber_Long(v);
+    if (!i) throw PyError{};
+    x = PyLong_AsLongLongAndOverflow(i, &over);
+    Py_DECREF(i);
+  }
   if (x == -1 && !over && PyErr_Occurred()) throw PyError{};
   if (over || x < static_cast<long long>(std::numeric_limits<T>::min()) || x > static_cast<long long>(std::numeric_limits<T>::max())) {
     PyErr_Format(PyExc_ValueError, "%s: a number out of range", what);
