@@ -325,8 +325,8 @@ __device__ __forceinline__ void norm_result(double* result, double v, int add) {
 constexpr int64_t kKeepBytes = int64_t(192) << 20;
 
 // One pass over the list.  A workgroup sums every gridDim.x-th tile and leaves one partial sum; the last to arrive joins them in
-// their order, so the result does not depend on who that is.  Bound by memory: 604 MB at 6.3 TB/s, 102 MB in 161 tensors 19.3 us (5.3
-// TB/s, of which about 4 us are the launch and the hand-over).  The hand-over is a store, a wait and an atomic of agent scope.
+// their order, so the result does not depend on who that is.  Bound by memory: 604 MB at 6.3 TB/s, 102 MB in 161 tensors 20.1 us
+// (5.1 TB/s, of which about 4 us are the launch and the hand-over), and 18.3 where the Infinity Cache holds them.  The hand-over is a store, a wait and an atomic of agent scope.
 // Stores of that scope are written through, so the wait for their acknowledgement orders them before the atomic; a release fence,
 // which also writes the L2 cache back, took 45 us more with 2048 workgroups.  Atomics on one address are served about 10 ns apart,
 // hence groups: 102 MB took 28 us with 1024 arrivals at one counter, 20.5 with 16 counters and another for them.  (512 workgroups of 512
@@ -467,9 +467,11 @@ __device__ __forceinline__ void clip_tile(const ClipSeg& sg, int64_t n, int64_t 
 // Second pass of a clipping call.  With `slots` the pass before has left its partial sums and nobody has joined them: every
 // workgroup does that for itself while its gradients are on the way, which saves the hand-over at the end of that pass and costs 4 KiB
 // of loads in each.  With / without, norm and clipping: 3 M fp16 elements (1500 tiles) 9.7 / 10.9 us, 10 M fp32 (4900) 22.0 / 23.5, 22 M
-// (10 700) 41.7 / 43.1, 100 M (48 800) 179.4 / 181.8, 302 M bf16 (147 500) 376.7 / 371.5.
-// Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 28.8 us (7.1 TB/s read and written), 110 M of a mixed
-// list 92 (7.2 TB/s).
+// (10 700) 41.7 / 43.1, 100 M (48 800) 178.6 / 180.1, bf16 116.7 / 118.4; 134 M (65 400) 239.6 / 242.5, bf16 160.1 / 160.7; 160 M (78 100)
+// 286.8 / 287.3, bf16 192.5 / 192.3; 200 M (97 700) 360.0 / 359.5, bf16 243.8 / 241.9; 302 M (147 500) 550.5 / 545.7, bf16 378.6 / 370.0.  (In place the
+// few workgroups join at every size: 134 M 258.9 / 259.3, 302 M 602.2 / 605.2, bf16 297.4 / 298.7, a gain that a rule of its own is not worth.)
+// Bound by what Infinity Cache and memory deliver together: 25.6 M fp32 elements 28.8 us behind their norm (7.1 TB/s read and written),
+// 35.0 where they come from memory (5.8); 110 M of a mixed list 92 (7.2 TB/s) and 109.7 (6.0).
 constexpr int64_t kJoinTiles = 65536;
 //
 // In place there may be nothing to do, so the coefficient comes first and the tiles are shared by few workgroups: 110 M elements of a mixed
