@@ -170,3 +170,51 @@ def test_sum_of_a_clip_that_measures(pkg, sizes, kind):
     assert abs(c - coefficient(math.sqrt(of_clip), 0.01)) <= abs(c) * 2.0 ** -24 * (1 + 1e-6)
     (a, b, length), = most
     assert a == b == length
+
+
+@pytest.mark.parametrize("which", ["tiny", "many", "large"])
+def test_every_call_captured(pkg, which):
+    # short lists, several tables, long lists; replayed four times with other gradients each, eager work between
+    sizes = SIZES[which]
+    types = types_of("mixed", sizes)
+    side = torch.cuda.Stream()
+
+    def fresh(seed):
+        return make(sizes, types, seed)[0], [make(sizes, ["fp32"] * len(sizes), seed + k)[0] for k in (1, 2, 3)]
+
+    index = [list(range(0, n, 3))[:50] for n in sizes]
+    msgs = [message(i) for i in index]
+    rooms = [m.numel() for m in msgs]
+    counts = torch.zeros(len(sizes), dtype=torch.int32, device="cuda")
+
+    def calls(g, out, u, d, results):
+        pkg.hp_cuda_grad_clip(g, sizes, out, 0.02, results[0], scale=0.5)
+        pkg.hp_cuda_grad_norm(g, sizes, results[1])
+        pkg.hp_cuda_grad_norm(out, sizes, results[1], is_add_to=1)
+        pkg.hp_cuda_gd_momentum(g, sizes, u, d, 0.9, 0.02, results[1])
+        pkg.hp_cuda_gd_mask(msgs, rooms, u, sizes, counts)
+        pkg.hp_cuda_grad_clip(g, sizes, None, 0.01, results[1], is_measured=1)
+        pkg.hp_cuda_grad_clip(g, sizes, None, math.inf, results[2], scale=-0.5)
+
+    g, (out, u, d) = fresh(200)
+    results = [pkg.hp_cuda_grad_result() for _ in range(3)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            calls(g, out, u, d, results)
+    held = [*g, *out, *u, *d]
+    for rep in range(4):
+        g2, (out2, u2, d2) = fresh(210 + 10 * rep)
+        eager = [pkg.hp_cuda_grad_result() for _ in range(3)]
+        for a, b in zip(held, [*g2, *out2, *u2, *d2]):
+            a.copy_(b)
+        calls(g2, out2, u2, d2, eager)
+        counts.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, [*g2, *out2, *u2, *d2])), rep
+        assert all(torch.equal(a[:3], b[:3]) for a, b in zip(results, eager)) and results[2][2].item() == -0.5
+        assert counts.tolist() == [len(i) for i in index]
+        assert math.isfinite(float(torch.randn(1 << 20, device="cuda").sum()))

@@ -857,6 +857,9 @@ struct Outs {
   int item(int type) const { return p ? 4 : item_size(type); }
 };
 
+static_assert(kPartElements % (kThreads * 4 * kClipIters) == 0 && kPartElements % (kThreads * 4 * kMomentumIters<false>) == 0 &&
+                  kPartElements / (kThreads * 4 * std::min(kClipIters, kMomentumIters<true>)) + 1 <= most_tiles(kThreads),
+              "a part begins on the tensor's place in a tile, and goes into a table");
 template <int ORDER, bool STREAM, int CAP>
 int launch_clip(int count, const void* const* grads, const int64_t* sizes, const int32_t* types, Outs outs, Clip clip, double* result, int slots, hipStream_t st) {
   return for_tables<ClipSeg, CAP>(
